@@ -54,7 +54,7 @@ struct ScwArgs {
   uint8_t *k, *v;
   float *ks, *vs;
   const int *table, *token_seq, *token_pos;
-  int n_split, width, n_seqs, n_pages, n_rot, n_angles, n_tokens, H, G, D, warps;
+  int n_split, width, n_seqs, n_pages, n_rot, n_angles, n_tokens, H, G, D, warps, settled;
   float eps, inv_d;
 };
 
@@ -69,6 +69,7 @@ __global__ void __launch_bounds__(SCW_WARPS * 32, sizeof(TIN) == 2 && SPW > 1 ? 
   const unsigned unit = blockIdx.x * SCW_WARPS + warp;              // a.warps warps share a token
   const int t = (int)(unit / (unsigned)a.warps), first = (int)(unit % (unsigned)a.warps) * SPW * HPW;
   if (t >= a.n_tokens) return;
+  if (!a.settled) pdl_wait();                       // the launch before may be what writes sequences and positions
   const int seq = a.token_seq[t], pos = a.token_pos[t];
   const int d0 = 4 * l, mid = D >> 1;               // dims d0 .. d0 + 3 and mid + d0 .. mid + d0 + 3
   const bool own = d0 < mid;
@@ -200,13 +201,14 @@ static int launch_write_by_head(const ScwArgs& a, cudaStream_t stream) {
 }
 
 // qkv: float32 or bfloat16 [T, (H+2G)*D], or n_split such float32 partials split_stride elements apart.  fmt: 0 int8, 1 e4m3.
-// D: a multiple of 16 up to 256.  cos_t, sin_t: [n_angles, n_rot / 2], a row per position.
+// D: a multiple of 16 up to 256.  cos_t, sin_t: [n_angles, n_rot / 2], a row per position.  settled: nothing that is still
+// running writes token_seq or token_pos.
 LLMX_API int llmx_scaled_cache_write(const void* qkv, int in_dtype, int n_split, long long split_stride, void* q_out,
                                      int act_dtype, void* k, void* v, float* k_scale, float* v_scale, int fmt,
                                      long long n_pages, const int* block_table, int table_width, int n_seqs,
                                      const int* token_seq, const int* token_pos, const float* q_gain, const float* k_gain,
                                      float eps, const float* cos_t, const float* sin_t, int n_rot, int n_angles, int n_tokens, int H, int G,
-                                     int D, const float* bias, cudaStream_t stream) {
+                                     int D, const float* bias, int settled, cudaStream_t stream) {
   if (n_tokens <= 0) return 0;
   if (H <= 0 || G <= 0 || D <= 0 || D > 256 || D % 16 || n_rot < 0 || n_rot > D || (n_rot & 1) || n_split < 1 || fmt < 0 || fmt > 1 ||
       n_pages <= 0 || n_pages > 0x7fffffff || table_width <= 0 || n_seqs <= 0)
@@ -220,7 +222,7 @@ LLMX_API int llmx_scaled_cache_write(const void* qkv, int in_dtype, int n_split,
   a.qkv = qkv, a.split_stride = split_stride, a.bias = bias, a.q_gain = q_gain, a.k_gain = k_gain, a.cos_t = cos_t, a.sin_t = sin_t;
   a.q_out = q_out, a.k = (uint8_t*)k, a.v = (uint8_t*)v, a.ks = k_scale, a.vs = v_scale;
   a.table = block_table, a.token_seq = token_seq, a.token_pos = token_pos;
-  a.n_split = n_split, a.width = table_width, a.n_seqs = n_seqs, a.n_pages = (int)n_pages, a.n_rot = n_rot, a.n_angles = n_angles, a.n_tokens = n_tokens, a.H = H, a.G = G, a.D = D;
+  a.n_split = n_split, a.width = table_width, a.n_seqs = n_seqs, a.n_pages = (int)n_pages, a.n_rot = n_rot, a.n_angles = n_angles, a.n_tokens = n_tokens, a.H = H, a.G = G, a.D = D, a.settled = settled;
   a.eps = eps, a.inv_d = 1.0f / (float)D;
 #define CASE(TIN, TA) return fmt == ROWS_INT8 ? launch_write_by_head<TIN, TA, ROWS_INT8>(a, stream) \
                                               : launch_write_by_head<TIN, TA, ROWS_E4M3>(a, stream)

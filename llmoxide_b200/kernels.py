@@ -1077,7 +1077,7 @@ _PV, _I, _L, _F = c_void_p, c_int, c_longlong, c_float
 _ROWS_ARGS = [_PV, _PV, _PV, _PV, _I, _L, _PV, _I]             # k, v, their scales, format, pages, block table, its width
 _SCALED_ARGS = {
     "llmx_scaled_cache_write": [_PV, _I, _I, _L, _PV, _I, *_ROWS_ARGS, _I, _PV, _PV, _PV, _PV, _F, _PV, _PV, _I, _I, _I, _I, _I, _I,
-                                _PV, _PV],
+                                _PV, _I, _PV],
     "llmx_scaled_cache_read": [*_ROWS_ARGS, _I, _PV, _PV, _PV, _PV, _I, _I, _I, _I, _PV],
     "llmx_scaled_attention_decode": [_PV, _PV, _I, *_ROWS_ARGS, _PV, _PV, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _PV],
     "llmx_scaled_attention_chunk": [_PV, _PV, _I, *_ROWS_ARGS, _PV, _PV, _PV, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _PV],
@@ -1132,13 +1132,16 @@ def _int32(name, t, dims: int, length: int = 0) -> None:
 
 
 def scaled_cache_write(qkv, q_out, k_cache, v_cache, k_scale, v_scale, block_table, token_seq, token_pos, q_gain, k_gain,
-                       eps: float, cos, sin, n_rot: int, n_heads: int, n_kv_heads: int, head_dim: int, bias=None) -> None:
+                       eps: float, cos, sin, n_rot: int, n_heads: int, n_kv_heads: int, head_dim: int, bias=None,
+                       settled: bool = False) -> None:
     """``qk_norm_rope_cache`` for a cache of 8-bit rows: qkv [T,(H+2G)*D], or float32 split partials [S,T,(H+2G)*D]
     summed in order, plus ``bias`` -> q_out [T,H*D] (normed, rotated) and k (normed, rotated) and v as rows of
     ``k_cache``/``v_cache`` [n_pages,G,PAGE,D] (int8 or float8_e4m3fn) with float32 scales ``k_scale``/``v_scale``
     [n_pages,G,PAGE] at each token's position.  A row x is held as round(x * (m / a)) with the scale a / m, a = max |x|,
     m = 127 (int8, ties to even) or 448 (e4m3); below a = 2^-100 as zeros with scale 0, and with an infinity or a NaN in it
-    as zeros with scale NaN.  float32 tokens from float32 or bfloat16 from either."""
+    as zeros with scale NaN.  float32 tokens from float32 or bfloat16 from either.  ``settled``: whatever wrote ``token_seq``
+    and ``token_pos`` has ended, so that they may be read while the launch before this one still runs (true of a step's,
+    which are copied ahead of its first launch)."""
     fmt = _scaled_cache(k_cache, v_cache, k_scale, v_scale, block_table, n_kv_heads, head_dim)
     shape, in_dtype, act_dtype = qkv.shape, qkv.dtype, q_out.dtype
     T, width, n_split, stride = shape[-2], (n_heads + 2 * n_kv_heads) * head_dim, 1, 0
@@ -1170,8 +1173,8 @@ def scaled_cache_write(qkv, q_out, k_cache, v_cache, k_scale, v_scale, block_tab
              k_scale.data_ptr(), v_scale.data_ptr(), fmt, k_cache.shape[0], block_table.data_ptr(), table[1], table[0],
              token_seq.data_ptr(), token_pos.data_ptr(), None if q_gain is None else q_gain.data_ptr(),
              None if k_gain is None else k_gain.data_ptr(), eps, cos.data_ptr() if n_rot else None,
-             sin.data_ptr() if n_rot else None, n_rot, angles, T, n_heads, n_kv_heads, head_dim, _ptr(bias), _stream()),
-           "scaled_cache_write")
+             sin.data_ptr() if n_rot else None, n_rot, angles, T, n_heads, n_kv_heads, head_dim, _ptr(bias), settled,
+             _stream()), "scaled_cache_write")
 
 
 def scaled_cache_read(k_cache, v_cache, k_scale, v_scale, block_table, token_seq, token_pos, k_out, v_out) -> None:

@@ -328,7 +328,7 @@ class GQAttention:
             if self.rows is not None and writes_cache:
                 kernels.scaled_cache_write(qkv, q, view.k, view.v, view.k_scale, view.v_scale, block_table, ctx.token_seq,
                                            ctx.token_pos, self.q_gain, self.k_gain, self.eps, cos, sin, n_rot, H, G, D,
-                                           bias=self.qkv_bias)
+                                           bias=self.qkv_bias, settled=True)
             else:
                 # (a call that only makes queries touches no cache: of 8-bit rows none is handed on)
                 k, v = (view.k, view.v) if self.rows is None else (q, q)
