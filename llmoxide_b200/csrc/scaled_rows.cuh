@@ -99,9 +99,10 @@ __device__ __forceinline__ uint32_t rows_bf16x2(float x, float y) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// The power of two that brings a magnitude to [2^target, 2^(target+1)), as far as float32 reaches, and its inverse.
+// The power of two that brings a magnitude to [2^target, 2^(target+1)), and its inverse; at most 2^118, so that the inverse is
+// a normal number with room for a further factor, and never 0.
 __device__ __forceinline__ void rows_power(float largest, int target, float& mul, float& inverse) {
-  const int e = min(254, target + 254 - (int)(__float_as_uint(largest) >> 23 & 255u));
+  const int e = min(245, target + 254 - (int)(__float_as_uint(largest) >> 23 & 255u));
   mul = __uint_as_float((uint32_t)e << 23), inverse = __uint_as_float((uint32_t)(254 - e) << 23);
 }
 #define ROWS_QUERY_POWER 13       // queries: largest of a row below 2^14

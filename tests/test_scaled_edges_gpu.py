@@ -5,7 +5,7 @@ test_scaled_cache_gpu.py."""
 import pytest
 import torch
 
-from test_scaled_cache_gpu import DEV, Cache, kernels, quantise, rows_of
+from test_scaled_cache_gpu import DEV, FMT, PAGE, Cache, attend, check, kernels, quantise, rows_of
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +38,57 @@ def test_positions_that_the_launch_before_makes(T):
             assert torch.equal(rows_of(store, c, seq, pos), held) and torch.equal(rows_of(scale, c, seq, pos), s)
             assert int((scale != 7.0).sum()) == T * G          # and nowhere else
     kernels().check_status()
+
+
+def attention_calls(D):
+    """(name, types of queries, call(q, out, cache, positions of sequences of one token)): single tokens and both kernels of several."""
+    def chunk(tc):
+        def run(q, out, c, pos, H, shares):
+            start = torch.arange(len(q) + 1, dtype=torch.int32, device=DEV)
+            kernels().scaled_attention_chunk(q, out, *c.args(), start, pos, len(q), 1, H, c.G, c.D, None, c.D ** -0.5, n_shares=shares, tc=tc)
+        return run
+
+    def decode(q, out, c, pos, H, shares):
+        kernels().scaled_attention_decode(q, out, *c.args(), pos, H, c.G, c.D, None, c.D ** -0.5, n_shares=shares)
+
+    both = (torch.bfloat16, torch.float32)
+    return [("decode", both, decode), ("chunk", both, chunk(False))] + ([("tcgen05", both[:1], chunk(True))] if D in (64, 128) else [])
+
+
+@pytest.mark.parametrize("fmt", list(FMT))
+@pytest.mark.parametrize("D", [64, 80, 128])
+def test_value_scales_of_next_to_nothing(D, fmt):
+    """A first page of scales of 2^-120 (no writer makes them, any caller may) ahead of ordinary ones: what they stand for is
+    nothing beside the rest, whatever the largest scale was when they were met."""
+    H, G, L = 4, 2, 200
+    c = Cache([L], G, D, fmt).fill()
+    page = int(c.table[0, 0])
+    c.V[0][:PAGE] *= 2.0 ** -120 / c.vs[page].T.double().unsqueeze(-1)
+    c.vs[page] = 2.0 ** -120
+    pos = torch.tensor([L - 1], dtype=torch.int32, device=DEV)
+    for name, dtypes, call in attention_calls(D):
+        for dtype in dtypes:
+            q = torch.randn(1, H * D, generator=torch.Generator(DEV).manual_seed(2), device=DEV).to(dtype)
+            want = attend(q.double().view(1, H, D), c.K[0], c.V[0], pos, None, 0, 0, D ** -0.5)
+            for shares in (1, 3):
+                out = torch.empty_like(q)
+                call(q, out, c, pos, H, shares)
+                check(out.view(1, H, D), *want, dtype, L)
+
+
+@pytest.mark.parametrize("D", [64, 80, 128])
+def test_queries_of_next_to_nothing(D):
+    """Queries of 2^-116 on keys of 2^115: their scores are ordinary."""
+    H, G, L = 4, 2, 100
+    c = Cache([L], G, D, "int8").fill()
+    for page in c.table[0].tolist():
+        c.ks[page] *= 2.0 ** 115
+    c.K[0] *= 2.0 ** 115
+    pos = torch.tensor([L - 1], dtype=torch.int32, device=DEV)
+    for name, dtypes, call in attention_calls(D):
+        for dtype in dtypes:
+            q = (torch.randn(1, H * D, generator=torch.Generator(DEV).manual_seed(2), device=DEV) * 2.0 ** -116).to(dtype)
+            want = attend(q.double().view(1, H, D), c.K[0], c.V[0], pos, None, 0, 0, D ** -0.5)
+            out = torch.empty_like(q)
+            call(q, out, c, pos, H, 1)
+            check(out.view(1, H, D), *want, dtype, L)
