@@ -5,8 +5,8 @@
 // the sequence's first keep_first ones, under a chunked mask of n those of its own n positions (floor(j/n) = floor(p/n));
 //   s_j = scale * ks_j * (q . k_j),  out = sum_j exp(s_j - m) vs_j v_j / sum_j exp(s_j - m),  m = max_j s_j
 // with k_j, v_j the held numbers and ks_j, vs_j their scales.  The held numbers are multiplied as float16, which is exact, and
-// so are bfloat16 queries (times a power of two a row).  The weights exp(s_j - m) vs_j are rounded once to float16: 2^-12 of
-// each, where the result's rounding to bfloat16 is 2^-9 on average.  float32 queries and weights go through the tensor cores as
+// so are bfloat16 queries (times a power of two a row).  The weights exp(s_j - r) vs_j, r a row's reference that follows its largest
+// weight (scaled_rows.cuh), are rounded once to float16: 2^-12 of each, where the result's rounding to bfloat16 is 2^-9 on average.  float32 queries and weights go through the tensor cores as
 // two float16 terms, 22 bits.  Scores, maxima, sums and accumulators are float32.  A token that sees no key gets zeros.
 //
 // A hidden key's scale is never multiplied: it may be anything (a page's former owner, or a NaN row outside the window).
@@ -97,8 +97,13 @@ struct SadSmem {
   static constexpr int TOTAL = RING > MERGE ? RING : MERGE;
 };
 
+// CTAs that fit a multiprocessor's registers.  (Its four quarters hold whole warps: at 133 registers three CTAs' 15 warps do not
+// fit, and 24 float32 tokens under a window of 1024 take 20 us instead of 14.5.)
+template <int DP, int TERMS, int NT>
+constexpr int sad_ctas() { return DP <= 64 ? 5 - NT : DP <= 128 ? 4 - NT : TERMS == 1 ? 2 : 1; }
+
 template <int DP, int FMT, int TERMS, int NT>
-__global__ void __launch_bounds__(SAD_THREADS)
+__global__ void __launch_bounds__(SAD_THREADS, sad_ctas<DP, TERMS, NT>())
 scaled_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SatArgs a) {
   using S = SadSmem<DP, NT>;
   constexpr int NU = DP / 64, NJ = DP / 16, HEADS = 8 * NT, NI = SAD_TILE / 16;
@@ -147,8 +152,7 @@ scaled_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   auto page_at = [&](int t) { return lo + t < n_kept ? lo + t : t_first + (lo + t - n_kept); };
 
   float o[NJ][NT][4];
-  float m[NT][2], l[NT][2];
-  float wmul = 0.f, winv = 0.f, wcap = 0.f;         // the weights' power of two, its inverse, the scale from which it is too large
+  float m[NT][2], l[NT][2];                         // what exponentials are taken against (ROWS_WEIGHT_POWER), their sum
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
@@ -273,7 +277,7 @@ scaled_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         }
 
       const bool edge = key0 + SAD_TILE - 1 > p || key0 < first;      // some key of the tile is hidden
-      float vscale[NI][2];
+      float vscale[NI][2], vlog[NI][2];
 #pragma unroll
       for (int i = 0; i < NI; ++i)
 #pragma unroll
@@ -281,37 +285,31 @@ scaled_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
           const int r = 16 * i + 8 * e + sg, key = key0 + r;
           const bool vis = !edge || ((key >= first || key < a.keep_first) && key <= p);
           const float kscale = sS[r], vs_here = sS[SAD_KEYS + r];
-          vscale[i][e] = vis ? vs_here : 0.f;
+          vscale[i][e] = vis ? vs_here : 0.f, vlog[i][e] = rows_log2(vs_here);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             s[i][n][2 * e] = vis ? s[i][n][2 * e] * (kscale * unit[n][0]) : -INFINITY;
             s[i][n][2 * e + 1] = vis ? s[i][n][2 * e + 1] * (kscale * unit[n][1]) : -INFINITY;
           }
         }
-      float grown = 1.f;
-      {
-        float vmax = 0.f;
-#pragma unroll
-        for (int i = 0; i < NI; ++i) vmax = fmaxf(vmax, fmaxf(vscale[i][0], vscale[i][1]));
-        if (__any_sync(0xffffffffu, vmax > wcap)) grown = sat_new_power(warp_max(vmax), wmul, winv, wcap);
-      }
-#pragma unroll
-      for (int i = 0; i < NI; ++i) vscale[i][0] *= wmul, vscale[i][1] *= wmul;
       uint32_t pb[NI][NT][TERMS][2];                 // P^T: keys 2 tq (+1) and + 8 of sixteen, head gq
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float mx0 = fmaxf(s[0][n][0], s[0][n][2]), mx1 = fmaxf(s[0][n][1], s[0][n][3]);
+        float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
-        for (int i = 1; i < NI; ++i) {
-          mx0 = fmaxf(mx0, fmaxf(s[i][n][0], s[i][n][2]));
-          mx1 = fmaxf(mx1, fmaxf(s[i][n][1], s[i][n][3]));
-        }
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            mx0 = fmaxf(mx0, s[i][n][2 * e] + vlog[i][e]);
+            mx1 = fmaxf(mx1, s[i][n][2 * e + 1] + vlog[i][e]);
+          }
 #pragma unroll
         for (int sh = 4; sh < 32; sh <<= 1) {
           mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, sh));
           mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, sh));
         }
-        mx0 = fmaxf(mx0, m[n][0]), mx1 = fmaxf(mx1, m[n][1]);      // (every tile walked has a visible key)
+        mx0 = fmaxf(mx0 - sat_weight_shift<TERMS>(), m[n][0]);     // (every tile walked has a visible key)
+        mx1 = fmaxf(mx1 - sat_weight_shift<TERMS>(), m[n][1]);
         const float c0 = sat_exp2<TERMS>(m[n][0] - mx0), c1 = sat_exp2<TERMS>(m[n][1] - mx1);
         m[n][0] = mx0, m[n][1] = mx1;
         float sum0 = 0.f, sum1 = 0.f;
@@ -322,14 +320,13 @@ scaled_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             const float e0 = sat_exp2<TERMS>(s[i][n][2 * e] - mx0), e1 = sat_exp2<TERMS>(s[i][n][2 * e + 1] - mx1);
             sum0 += e0, sum1 += e1;
             uint32_t terms[TERMS];
-            rows_split2<TERMS>(e0 * vscale[i][e], e1 * vscale[i][e], terms);
+            rows_split2<TERMS>(e0 * vscale[i][e] * sat_weight_mul<TERMS>(), e1 * vscale[i][e] * sat_weight_mul<TERMS>(), terms);
 #pragma unroll
             for (int u = 0; u < TERMS; ++u) pb[i][n][u][e] = sat_transpose(terms[u]);
           }
         l[n][0] = l[n][0] * c0 + sum0, l[n][1] = l[n][1] * c1 + sum1;
-        const float f0 = c0 * grown, f1 = c1 * grown;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) o[j][n][0] *= f0, o[j][n][1] *= f1, o[j][n][2] *= f0, o[j][n][3] *= f1;
+        for (int j = 0; j < NJ; ++j) o[j][n][0] *= c0, o[j][n][1] *= c1, o[j][n][2] *= c0, o[j][n][3] *= c1;
       }
 
       // O^T += V^T P^T: rows gq and gq + 8 of product j are neighbouring dims of the lane's 16 (DP 64: 8)
@@ -393,14 +390,15 @@ scaled_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   float* cacc = mml + SAD_WARPS * HEADS * 2;                                     // [HEADS][DP]: the CTA's, for its cluster
   float* cml = cacc + HEADS * DP;
   if (warp < SAD_WARPS) {
+  constexpr float back = 1.f / sat_weight_mul<TERMS>();
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const int hA = warp * HEADS + 8 * n + 2 * tq;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int d = DP == 64 ? 8 * gq + 2 * j : 128 * (j >> 3) + 16 * gq + 2 * (j & 7);
-      *reinterpret_cast<float2*>(macc + (size_t)hA * DP + d) = make_float2(o[j][n][0] * winv, o[j][n][2] * winv);
-      *reinterpret_cast<float2*>(macc + (size_t)(hA + 1) * DP + d) = make_float2(o[j][n][1] * winv, o[j][n][3] * winv);
+      *reinterpret_cast<float2*>(macc + (size_t)hA * DP + d) = make_float2(o[j][n][0] * back, o[j][n][2] * back);
+      *reinterpret_cast<float2*>(macc + (size_t)(hA + 1) * DP + d) = make_float2(o[j][n][1] * back, o[j][n][3] * back);
     }
     if (gq == 0) {
       mml[2 * hA] = m[n][0], mml[2 * hA + 1] = l[n][0];
@@ -663,7 +661,6 @@ __global__ void __launch_bounds__(SAC_WARPS * 32) scaled_chunk_kernel(const SatA
   __syncwarp();
 
   float o[NJ][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  float wmul = 0.f, winv = 0.f, wcap = 0.f;         // as in scaled_decode_kernel
 #pragma unroll
   for (int j = 0; j < NJ; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
   for (int t = 0; t < n_tiles; ++t) {
@@ -713,11 +710,13 @@ __global__ void __launch_bounds__(SAC_WARPS * 32) scaled_chunk_kernel(const SatA
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint2 kk = sat_lds64(sS + 4 * (8 * i + 2 * tq));
+      const uint2 vv = sat_lds64(sS + 4 * (SAC_KEYS + 8 * i + 2 * tq));
       const float k0 = __uint_as_float(kk.x), k1 = __uint_as_float(kk.y);
+      const float log0 = rows_log2(__uint_as_float(vv.x)), log1 = rows_log2(__uint_as_float(vv.y));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         s[i][e] = (seen >> (4 * i + e)) & 1u ? s[i][e] * ((e & 1 ? k1 : k0) * unit[e >> 1]) : -INFINITY;
-        mx[e >> 1] = fmaxf(mx[e >> 1], s[i][e]);
+        mx[e >> 1] = fmaxf(mx[e >> 1], s[i][e] + (e & 1 ? log1 : log0));
       }
     }
     float ref[2], c[2], sum[2] = {0.f, 0.f};
@@ -725,36 +724,27 @@ __global__ void __launch_bounds__(SAC_WARPS * 32) scaled_chunk_kernel(const SatA
     for (int r = 0; r < 2; ++r) {
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
       mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-      mx[r] = fmaxf(mx[r], m[r]);
+      mx[r] = fmaxf(mx[r] - sat_weight_shift<TERMS>(), m[r]);
       ref[r] = mx[r] == -INFINITY ? 0.f : mx[r];    // a row that has seen nothing yet
       c[r] = sat_exp2<TERMS>(m[r] - ref[r]);
       m[r] = mx[r];
     }
-    float grown = 1.f, vmax = 0.f;                  // the largest scale that a row of the warp sees
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint2 vv = sat_lds64(sS + 4 * (SAC_KEYS + 8 * i + 2 * tq));
-      if ((seen >> (4 * i)) & 5u) vmax = fmaxf(vmax, __uint_as_float(vv.x));
-      if ((seen >> (4 * i)) & 10u) vmax = fmaxf(vmax, __uint_as_float(vv.y));
-    }
-    if (__any_sync(0xffffffffu, vmax > wcap)) grown = sat_new_power(warp_max(vmax), wmul, winv, wcap);
-    const float f0 = c[0] * grown, f1 = c[1] * grown;
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) o[j][0] *= f0, o[j][1] *= f0, o[j][2] *= f1, o[j][3] *= f1;
+    for (int j = 0; j < NJ; ++j) o[j][0] *= c[0], o[j][1] *= c[0], o[j][2] *= c[1], o[j][3] *= c[1];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {                   // sixteen keys at a time
       uint32_t pa[TERMS][4];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const uint2 vv = sat_lds64(sS + 4 * (SAC_KEYS + 16 * i + 8 * x + 2 * tq));
-        const float w0 = __uint_as_float(vv.x) * wmul, w1 = __uint_as_float(vv.y) * wmul;
+        const float w0 = __uint_as_float(vv.x), w1 = __uint_as_float(vv.y);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const float p0 = sat_exp2<TERMS>(s[2 * i + x][2 * r] - ref[r]), p1 = sat_exp2<TERMS>(s[2 * i + x][2 * r + 1] - ref[r]);
           sum[r] += p0 + p1;
           const uint32_t vis = seen >> (4 * (2 * i + x) + 2 * r);
           uint32_t terms[TERMS];
-          rows_split2<TERMS>(vis & 1u ? p0 * w0 : 0.f, vis & 2u ? p1 * w1 : 0.f, terms);
+          rows_split2<TERMS>(vis & 1u ? p0 * w0 * sat_weight_mul<TERMS>() : 0.f, vis & 2u ? p1 * w1 * sat_weight_mul<TERMS>() : 0.f, terms);
 #pragma unroll
           for (int e = 0; e < TERMS; ++e) pa[e][2 * x + r] = terms[e];
         }
@@ -806,7 +796,7 @@ __global__ void __launch_bounds__(SAC_WARPS * 32) scaled_chunk_kernel(const SatA
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     if (!live[r]) continue;
     const size_t row = (size_t)(tok0 + token[r]) * H + head[r];
-    const float f = (a.n_split > 1 ? 1.f : l[r] == 0.f ? 0.f : 1.f / l[r]) * winv;
+    const float f = (a.n_split > 1 ? 1.f : l[r] == 0.f ? 0.f : 1.f / l[r]) / sat_weight_mul<TERMS>();
     float* part = a.ws + (row * a.n_split + share) * SAT_WS_ROW(D);
     constexpr int RUN = DP == 64 ? 8 : 16;          // neighbouring dims of a lane: columns 2 tq and 2 tq + 1 of the products
 #pragma unroll

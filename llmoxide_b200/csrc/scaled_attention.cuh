@@ -19,14 +19,10 @@ __device__ __forceinline__ float sat_largest(float top, float4 f) {
   const uint32_t b = max(__float_as_uint(f.z) & 0x7fffffffu, __float_as_uint(f.w) & 0x7fffffffu);
   return __uint_as_float(max(__float_as_uint(top), max(a, b)));
 }
-// A larger value scale has been seen: the power of two for the weights from here on, and what the accumulators so far are
-// multiplied by.  (Before the first there are none.)
-__device__ __forceinline__ float sat_new_power(float vmax, float& wmul, float& winv, float& wcap) {
-  const float before = winv;
-  rows_power(vmax, ROWS_WEIGHT_POWER, wmul, winv);
-  wcap = ROWS_WEIGHT_CAP * winv;
-  return before == 0.f ? 1.f : before * wmul;
-}
+// Weights at 2^13 (ROWS_WEIGHT_POWER): by the reference where they are rounded once; by a factor of its own where float32 is kept
+// in two terms, since an argument of the exponential that is larger by 13 costs it a digit and a half.
+template <int TERMS> __device__ __forceinline__ constexpr float sat_weight_shift() { return TERMS == 1 ? ROWS_WEIGHT_POWER : 0.f; }
+template <int TERMS> __device__ __forceinline__ constexpr float sat_weight_mul() { return TERMS == 1 ? 1.f : 8192.f; }
 
 struct SatArgs {
   const void* q;

@@ -1,18 +1,22 @@
 // Attention of several new tokens per sequence over the cache of 8-bit rows on the 5th-generation tensor cores (tcgen05):
-// bfloat16 queries, head sizes 64 and 128.  Formulas and roundings as in scaled_attention.cu.
+// bfloat16 queries, head sizes 64 and 128.  Formulas and roundings as in scaled_attention.cu, but for the weights' reference, which
+// lags: a row's largest weight lies between 2^10 and 2^15.5, so that weights below 2^-24 of it lose digits and those below
+// 2^-35 vanish.
 //
 // Rows of the product are a kv head's (token, query head) pairs, token after token, so that the heads that share keys share a
 // tile, and a few tokens fill it.  A CTA owns 256 of them, as two tiles of 128 (a row = a lane of tensor memory), and walks the
 // visible keys a page of 64 at a time:
 //   warp 0       bulk copies: a page's 8-bit keys and values and their scales, each one stretch of memory, into two stages
 //   warps 4-7    make them float16 in the layout the tensor cores read (128-byte swizzle), for both tiles at once; one of
-//                them follows the largest value scale and brings the values' scales to the weights' power of two
+//                them lays out the page's scales, the logarithms of the values' and that of the largest
 //   warps 1, 2   for a tile each, one lane issues S = Q K^T into one of two buffers in tensor memory, and O += P V, P from tensor
 //                memory.  (One lane for both: the tensor cores take no product ahead of the one they work on, and idle while it
 //                waits or commits; 900 of 2230 cycles a page without any softmax.)
-//   warps 8-23   softmax, two threads a row, 32 keys each: scores times the keys' scales, running maximum, exp2, sum, the weights
-//                times the values' scales as float16 back over the scores they came from.  O is rescaled in tensor memory only
-//                when a row's maximum has grown by 2^4, or the weights' power of two has changed.
+//   warps 8-23   softmax, two threads a row, 32 keys each: scores times the keys' scales, their maximum, exp2, sum, the weights
+//                times the values' scales as float16 back over the scores they came from.  The largest score and the page's
+//                largest value scale bound a page's weights; only where that bound is 2^5.5 above the row's reference is the
+//                largest weight itself looked for (one page in 60 of random ones), and O is rescaled in tensor memory
+//                only where that has grown by as much.
 // Converting a page is 16384 numbers at five instructions for four (int8), once for 256 rows.  The numbers of a group of four
 // lie in the order that conversion gives, in the queries too; the result's columns are put back at the end.
 // With n_split > 1 the walk is cut into shares, whose partials meet in scaled_merge_kernel.
@@ -27,9 +31,8 @@
 #define STC_HALF (STC_KEYS / 2)
 #define STC_THREADS 768
 #define STC_MAX_SPLIT 64
-#define STC_LAG 4.0f                 // a row's maximum may outgrow the one its exponentials are taken against by 2^4
-#define STC_WEIGHT_POWER 9           // so weights are below 2^4 times the scales' 2^11
-#define STC_WEIGHT_CAP 2048.f
+#define STC_LAG 5.5f                 // a row's largest weight may outgrow the one it is taken against by 2^5.5,
+#define STC_WEIGHT_POWER 10.f        // which comes to 2^10: below 2^15.5, float16 ends at 2^16
 
 template <int D>
 struct StcSmem {
@@ -38,8 +41,8 @@ struct StcSmem {
   static constexpr int RAW = STC_KEYS * D;                        // 8 bits
   static constexpr int K = 2 * QTILE, V = K + 2 * TILE;
   static constexpr int RAW0 = V + 2 * TILE, RAW_STAGE = 2 * RAW + 2 * STC_KEYS * 4;      // K, V, scales of K, scales of V
-  static constexpr int SCALES = RAW0 + 2 * RAW_STAGE;             // [4 slots]: scales of K [64], of V in weights [64], 4 words
-  static constexpr int SLOT = 2 * STC_KEYS * 4 + 16;              // words: what accumulators grow by, the inverse power
+  static constexpr int SCALES = RAW0 + 2 * RAW_STAGE;             // [4 slots]: scales of K [64], of V [64], log2 of V's [64], 4 words
+  static constexpr int SLOT = 3 * STC_KEYS * 4 + 16;              // words: log2 of the largest scale of V
   static constexpr int TOLD = SCALES + 4 * SLOT;                  // [2 tiles][2][128]: what the two threads of a row tell each other
   static constexpr int BARS = TOLD + 2 * 2 * 128 * 4;
   static constexpr int TOTAL = BARS + 32 * 8;
@@ -251,7 +254,6 @@ __global__ void __launch_bounds__(STC_THREADS, 1) scaled_chunk_tc_kernel(const S
   } else if (warp >= 4 && warp < 8) {
     // ---------------- conversion ----------------
     const int t = threadIdx.x - 128;
-    float wmul = 0.f, winv = 0.f, wcap = 0.f;
     int gave_up = 0;                 // which wait ran out for this thread; looked at once a tile
     auto wait = [&](uint32_t bar, uint32_t parity, int code) {
       if (!mbar_wait(bar, parity)) gave_up = code;
@@ -276,18 +278,15 @@ __global__ void __launch_bounds__(STC_THREADS, 1) scaled_chunk_tc_kernel(const S
           const int key = key0 + lane + 32 * e;
           const bool vis = key <= pos_hi && (key >= first_lo || key < a.keep_first);
           v[e] = vis ? from[STC_KEYS + lane + 32 * e] : 0.f;
-          vmax = fmaxf(vmax, v[e]);
+          vmax = fmaxf(vmax, fabsf(v[e]));
         }
-        float grown = 1.f;
-        if (__any_sync(0xffffffffu, vmax > wcap)) {
-          const float before = winv;
-          rows_power(warp_max(vmax), STC_WEIGHT_POWER, wmul, winv);
-          wcap = STC_WEIGHT_CAP * winv;
-          grown = before == 0.f ? 1.f : before * wmul;
-        }
+        const float largest = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vmax)));      // (no number below 0)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) to[lane + 32 * e] = from[lane + 32 * e], to[STC_KEYS + lane + 32 * e] = v[e] * wmul;
-        if (lane == 0) to[2 * STC_KEYS] = grown, to[2 * STC_KEYS + 1] = winv;
+        for (int e = 0; e < 2; ++e) {
+          to[lane + 32 * e] = from[lane + 32 * e], to[STC_KEYS + lane + 32 * e] = v[e];
+          to[2 * STC_KEYS + lane + 32 * e] = rows_log2(v[e]);
+        }
+        if (lane == 0) to[3 * STC_KEYS] = rows_log2(largest);
         __syncwarp();
         if (lane == 0) mbar_arrive(scales_ready + 8 * (j & 3));
       }
@@ -365,8 +364,8 @@ __global__ void __launch_bounds__(STC_THREADS, 1) scaled_chunk_tc_kernel(const S
     const int edge_hi = pos_lo - (STC_KEYS - 1);
     int edge_lo = a.window > 0 ? pos_hi - (a.window - 1) : 0;
     if (a.mask_chunk > 0) edge_lo = max(edge_lo, pos_hi - pos_hi % a.mask_chunk);
-    float m_used = -INFINITY;        // the maximum the exponentials are taken against; of both threads
-    float l = 0.f, winv = 0.f;       // this thread's share of the row sum in units of 2^-m_used
+    float m_used = -INFINITY;        // log2 of the row's largest weight (probability times scale), a while ago; of both threads
+    float l = 0.f;                   // this thread's share of the row sum in units of 2^(m_used - STC_WEIGHT_POWER)
     bool left = false;
     int gave_up = 0;                 // which wait ran out for this thread; looked at once a tile
     auto wait = [&](uint32_t bar, uint32_t parity, int code) {
@@ -385,9 +384,7 @@ __global__ void __launch_bounds__(STC_THREADS, 1) scaled_chunk_tc_kernel(const S
       wait(pair_bar(s_full, x, st), (j >> 1) & 1, 13);
       tc_fence_after();
       tmem_ld32_nowait(tS_row + (uint32_t)(half * STC_HALF), sr);
-      const float2 power = *reinterpret_cast<const float2*>(slot + 2 * STC_KEYS);
-      const float grown = power.x;
-      winv = power.y;
+      const float loudest = slot[3 * STC_KEYS];
       tmem_ld_wait();
       const float4* ks = reinterpret_cast<const float4*>(slot + half * STC_HALF);
 #pragma unroll
@@ -413,9 +410,23 @@ __global__ void __launch_bounds__(STC_THREADS, 1) scaled_chunk_tc_kernel(const S
         mx2[0] = stc_max3(mx2[0], __uint_as_float(sr[e]), __uint_as_float(sr[e + 1]));
         mx2[1] = stc_max3(mx2[1], __uint_as_float(sr[e + 2]), __uint_as_float(sr[e + 3]));
       }
-      float mt = fmaxf(mx2[0], mx2[1]) * unit;       // unit > 0
+      // no weight of the tile is above this: unit > 0
+      float mt = fmaf(fmaxf(mx2[0], mx2[1]), unit, loudest);
       tc_fence_before();           // (the other warp's P goes over scores that this one has read, and the other way round)
-      if (stc_pair_any(id, gave_up || mt > m_used + STC_LAG || grown != 1.f)) {    // also the first time (m_used = -inf)
+      if (stc_pair_any(id, gave_up || mt > m_used + STC_LAG)) {    // also the first time (m_used = -inf)
+        // the largest weight itself: the loudest value may be another key's, or one that this row does not see.  (Looked for in
+        // every tile: 363 us for 2048 tokens after 6144, 340 so.)
+        const float4* logs = reinterpret_cast<const float4*>(slot + 2 * STC_KEYS + half * STC_HALF);
+        mt = -INFINITY;
+        const f32x2 unit_2 = stc_pack(unit, unit);
+#pragma unroll
+        for (int e = 0; e < STC_HALF; e += 4) {
+          const float4 w = logs[e / 4];
+          const f32x2 u = stc_fma2(stc_pack(__uint_as_float(sr[e]), __uint_as_float(sr[e + 1])), unit_2, stc_pack(w.x, w.y));
+          const f32x2 v = stc_fma2(stc_pack(__uint_as_float(sr[e + 2]), __uint_as_float(sr[e + 3])), unit_2, stc_pack(w.z, w.w));
+          mt = stc_max3(mt, stc_lo(u), stc_hi(u));
+          mt = stc_max3(mt, stc_lo(v), stc_hi(v));
+        }
         told[half * 128 + row] = mt;
         if (stc_pair_any(id, gave_up)) {
           left = true;
@@ -429,7 +440,6 @@ __global__ void __launch_bounds__(STC_THREADS, 1) scaled_chunk_tc_kernel(const S
           m_used = mt;
         }
         l *= alpha;
-        alpha *= grown;
         if (j >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
           wait(pair_bar(pv_done, x, (j - 1) & 1), ((j - 1) >> 1) & 1, 14);
           tc_fence_after();
@@ -447,7 +457,7 @@ __global__ void __launch_bounds__(STC_THREADS, 1) scaled_chunk_tc_kernel(const S
       } else {
         tc_fence_after();
       }
-      const float ref = m_used == -INFINITY ? 0.f : -m_used;
+      const float ref = m_used == -INFINITY ? 0.f : STC_WEIGHT_POWER - m_used;
       const f32x2 unit2 = stc_pack(unit, unit), ref2 = stc_pack(ref, ref);
       const float4* vs = reinterpret_cast<const float4*>(slot + STC_KEYS + half * STC_HALF);
       f32x2 sum2[2] = {0ull, 0ull};
@@ -484,7 +494,7 @@ __global__ void __launch_bounds__(STC_THREADS, 1) scaled_chunk_tc_kernel(const S
     if (!left && !stc_pair_any(id, gave_up)) {
       l = told[row] + told[128 + row];
       const size_t at = (size_t)(tok0 + token) * H + head;
-      const float f = (a.n_split > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l) * winv;
+      const float f = a.n_split > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
       float* part = a.ws + (at * a.n_split + share) * SAT_WS_ROW(D);
       constexpr int I1 = rows_second<FMT>() == 2 ? 2 : 1, I2 = 3 - I1;       // where dims 1 and 2 of four lie
 #pragma unroll 1
@@ -510,7 +520,7 @@ __global__ void __launch_bounds__(STC_THREADS, 1) scaled_chunk_tc_kernel(const S
           }
         }
       }
-      if (live && a.n_split > 1 && half == 0) part[D] = m_used, part[D + 1] = l;
+      if (live && a.n_split > 1 && half == 0) part[D] = m_used - STC_WEIGHT_POWER, part[D + 1] = l;
     }
   }
   tc_fence_before();

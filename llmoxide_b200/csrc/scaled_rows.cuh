@@ -7,8 +7,8 @@
 //
 // The attention kernels multiply the held numbers as float16, which holds each of them exactly (8 and 4 significant bits), and
 // apply the scales to the float32 scores and probabilities.  What meets them in a product is float16 too: queries times a
-// power of two a row, chosen so that bfloat16 queries stay exact, and probabilities with the values' scales in them, times a
-// power of two that follows the largest scale seen, rounded to 11 bits.  float16 rather than bfloat16: three bits more in
+// power of two a row, chosen so that bfloat16 queries stay exact, and probabilities with the values' scales in them, relative
+// to the row's largest such weight, rounded to 11 bits.  float16 rather than bfloat16: three bits more in
 // the probabilities, and two instructions a pair of int8 numbers where bfloat16 takes three.
 #pragma once
 
@@ -106,11 +106,20 @@ __device__ __forceinline__ void rows_power(float largest, int target, float& mul
   mul = __uint_as_float((uint32_t)e << 23), inverse = __uint_as_float((uint32_t)(254 - e) << 23);
 }
 #define ROWS_QUERY_POWER 13       // queries: largest of a row below 2^14
-// Probabilities (at most 1) times the values' scales: a scale's power is chosen at 2^13, and again when a larger one reaches
-// 2^15; float16 ends at 2^16, and steps by 2^-24 at its lower end: a weight below 2^-27 of the largest scale loses digits, one
-// below 2^-38 vanishes.
-#define ROWS_WEIGHT_POWER 13
-#define ROWS_WEIGHT_CAP 32768.f
+// Weights: exp(s_j - r) vs_j, the probability of a key with its value's scale in it.  The reference r of a row follows the
+// largest s_j + log(vs_j) that the row sees, not the largest s_j, so that the largest weight comes to 2^13 whatever the
+// scales: float16 ends at 2^16 and steps by 2^-24 at its lower end, so a weight 2^-27 of the row's largest loses digits and one
+// below 2^-38 vanishes, and neither a key that a row does not see nor one that it gives no weight has a say in that.  The
+// row's sum of exp(s_j - r) goes by the same reference, which leaves it far from float32's ends: r is off the largest s_j by the
+// log of one scale.
+#define ROWS_WEIGHT_POWER 13.f
+// log2 of a value's scale, for that reference.  A scale of zeros, or of next to nothing, counts as 2^-96: the sum of such a
+// row's exponentials stays finite.
+__device__ __forceinline__ float rows_log2(float scale) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fabsf(scale)));
+  return fmaxf(y, -96.f);                          // (also for a NaN, which the weight itself carries on)
+}
 
 // The bytes [rows, cols] of a cache, in boxes of [box_rows x box_cols], laid down with the swizzle of box_cols bytes
 // (64 or 128; none with `plain`).

@@ -92,3 +92,63 @@ def test_queries_of_next_to_nothing(D):
             out = torch.empty_like(q)
             call(q, out, c, pos, H, 1)
             check(out.view(1, H, D), *want, dtype, L)
+
+
+@pytest.mark.parametrize("fmt", list(FMT))
+@pytest.mark.parametrize("window", [None, 40])
+@pytest.mark.parametrize("D, tc", [(64, False), (80, False), (128, False), (64, True), (128, True)])
+def test_a_loud_row_is_nothing_to_those_that_do_not_see_it(D, tc, window, fmt):
+    """One value row of a scale 2^40 above the others: whoever does not see it gets, bit for bit, what it got without it."""
+    H, G, L, n = 4, 2, 330, 300
+    c = Cache([L], G, D, fmt).fill()
+    start, past = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([0, n], [L - n]))
+    for dtype in (torch.bfloat16,) if tc else (torch.bfloat16, torch.float32):
+        q = torch.randn(n, H * D, generator=torch.Generator(DEV).manual_seed(5), device=DEV).to(dtype)
+        run = lambda out: kernels().scaled_attention_chunk(q, out, *c.args(), start, past, 1, n, H, G, D, window, D ** -0.5, n_shares=1, tc=tc)
+        clean = torch.empty_like(q)
+        run(clean)
+        for bad in (60, 191, 300, L - 1):
+            page, row = int(c.table[0, bad // PAGE]), bad % PAGE
+            scale, values = c.vs[page, :, row].clone(), c.V[0][bad].clone()
+            c.vs[page, :, row] *= 2.0 ** 40
+            c.V[0][bad] *= 2.0 ** 40
+            out = torch.empty_like(q)
+            run(out)
+            want = attend(q.double().view(n, H, D), c.K[0], c.V[0], torch.arange(L - n, L, device=DEV), window, 0, 0, D ** -0.5)
+            c.vs[page, :, row], c.V[0][bad] = scale, values
+            at = torch.arange(L - n, L, device=DEV)
+            sees = (at >= bad) & (at < bad + (window or L))
+            assert torch.equal(out[~sees], clean[~sees]), (bad, dtype)
+            if sees.any():
+                check(out[sees].view(-1, H, D), *(x[sees] for x in want), dtype, L)
+
+
+@pytest.mark.parametrize("fmt", list(FMT))
+@pytest.mark.parametrize("D", [64, 80, 128])
+def test_a_loud_row_that_nobody_weighs(D, fmt):
+    """A visible value row 2^30 above the others under a key whose weight is about 2^-60 of the others': they keep their digits.
+    What a weight loses at float16's end goes by the row's largest product of probability and value, not by the largest value:
+    2^-38 of it, and on tcgen05, whose largest weight is kept above 2^10 and not 2^13, 2^-35."""
+    H, G, L, loud = 4, 2, 700, 130
+    c = Cache([L], G, D, fmt).fill(strength=0.5)
+    q0 = torch.randn(D, generator=torch.Generator(DEV).manual_seed(8), device=DEV)
+    page, row = int(c.table[0, loud // PAGE]), loud % PAGE
+    key = (-42.0 * D ** 0.5 / (q0 @ q0) * q0).expand(G, D)
+    held, scale = quantise(key, fmt)
+    c.k.view(torch.int8)[page, :, row], c.ks[page, :, row] = held.view(torch.int8), scale
+    c.K[0][loud] = held.float().double() * scale.double().unsqueeze(-1)
+    c.vs[page, :, row] *= 2.0 ** 30
+    c.V[0][loud] *= 2.0 ** 30
+    pos = torch.tensor([L - 1], dtype=torch.int32, device=DEV)
+    for name, dtypes, call in attention_calls(D):
+        for dtype in dtypes:
+            q = q0.expand(H, D).reshape(1, H * D).to(dtype)
+            x = q.double().view(1, H, D)
+            out64, mag, score, _ = attend(x, c.K[0], c.V[0], pos, None, 0, 0, D ** -0.5)
+            p = [torch.softmax(c.K[0][:, h // (H // G)] @ x[0, h] * D ** -0.5, 0) for h in range(H)]
+            assert all(2.0 ** -68 < float(y[loud] / y.max()) < 2.0 ** -50 for y in p)
+            largest = torch.stack([(y * c.V[0][:, h // (H // G)].abs().amax(-1)).max() for h, y in enumerate(p)]).view(1, H, 1)
+            for shares in (1, 3):
+                out = torch.empty_like(q)
+                call(q, out, c, pos, H, shares)
+                check(out.view(1, H, D), out64, mag, score, largest * (8 if name == "tcgen05" else 1), dtype, L)
