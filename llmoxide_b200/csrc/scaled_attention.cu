@@ -528,7 +528,7 @@ LLMX_API int llmx_scaled_attention_decode(const void* q, void* out, int f32, con
                                           cudaStream_t stream) {
   if (B <= 0) return 0;
   const SatArgs a = sat_args(q, out, k, v, k_scale, v_scale, n_pages, block_table, table_width, nullptr, seq_past, ws, H, G, D, window,
-                             keep_first, mask_chunk, scale, n_split, 0, settled);
+                             keep_first, mask_chunk, scale, n_split, B, 1, settled);
   if (int code = sat_refuse(a, fmt, f32, SAD_MAX_SPLIT)) return code;
   if (n_split > SAD_CLUSTER && !ws) return LLMX_REFUSED(1);
   if (B > 65535) return LLMX_REFUSED(3);
@@ -572,10 +572,11 @@ __global__ void __launch_bounds__(SAC_WARPS * 32) scaled_chunk_kernel(const SatA
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gq = lane >> 2, tq = lane & 3;
   const int b = blockIdx.z, H = a.H, G = a.G, D = a.D, R = H / G;
   const int g = blockIdx.y / a.n_split, share = blockIdx.y % a.n_split;
-  const int tok0 = a.seq_start[b], n_new = a.seq_start[b + 1] - tok0, n_rows = n_new * R;
+  int tok0, n_new, past;
+  sat_tokens(a, b, tok0, n_new, past);
+  const int n_rows = n_new * R;
   const int row0 = (gridDim.x - 1 - blockIdx.x) * SAC_ROWS;          // the longest walks first
   if (row0 >= n_rows) return;
-  const int past = a.seq_past[b];
   const int pos_lo = past + row0 / R, pos_hi = past + (min(row0 + SAC_ROWS, n_rows) - 1) / R;
   int first_lo = (a.window > 0 && pos_lo - (a.window - 1) > 0) ? pos_lo - (a.window - 1) : 0;
   if (a.mask_chunk > 0) first_lo = max(first_lo, pos_lo - pos_lo % a.mask_chunk);
@@ -840,7 +841,7 @@ LLMX_API int llmx_scaled_attention_chunk(const void* q, void* out, int f32, cons
   if (B <= 0 || T <= 0 || max_new <= 0) return 0;
   if (G <= 0 || H <= 0 || (long long)max_new * (H / G) > 0x7fffffff - SAC_ROWS) return LLMX_REFUSED(3);
   const SatArgs a = sat_args(q, out, k, v, k_scale, v_scale, n_pages, block_table, table_width, seq_start, seq_past, ws, H, G, D, window,
-                             keep_first, mask_chunk, scale, n_split, max_new * (H / G), 0);
+                             keep_first, mask_chunk, scale, n_split, T, max_new, 0);
   if (int code = sat_refuse(a, fmt, f32, SAC_MAX_SPLIT)) return code;
   if (n_split > 1 && !ws) return LLMX_REFUSED(1);
   if (B > 65535 || (long long)G * n_split > 65535) return LLMX_REFUSED(3);

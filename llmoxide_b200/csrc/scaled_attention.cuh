@@ -31,7 +31,7 @@ struct SatArgs {
   const float *ks, *vs;
   const int *table, *seq_start, *seq_past;
   float* ws;
-  int width, n_pages, H, G, D, window, keep_first, mask_chunk, n_split, tensor_copies, max_rows, settled;
+  int width, n_pages, H, G, D, window, keep_first, mask_chunk, n_split, tensor_copies, max_rows, settled, n_tokens, max_new;
   float scale_log2;
 };
 __device__ __forceinline__ int sat_checked(const SatArgs& a, int p) {
@@ -41,6 +41,18 @@ __device__ __forceinline__ int sat_checked(const SatArgs& a, int p) {
 }
 __device__ __forceinline__ int sat_page(const SatArgs& a, const int* pages, int logical) {
   return sat_checked(a, logical < a.width ? pages[logical] : -1);
+}
+
+// Several tokens a sequence: those of sequence b and their first position, both inside the launch's arrays; a sequence that is not
+// has none, and is reported.
+__device__ __forceinline__ void sat_tokens(const SatArgs& a, int b, int& tok0, int& n_new, int& past) {
+  const int end = a.seq_start[b + 1];
+  tok0 = a.seq_start[b], past = a.seq_past[b], n_new = 0;
+  if (tok0 >= 0 && end >= tok0 && end <= a.n_tokens && end - tok0 <= a.max_new &&
+      (end == tok0 || (past >= 0 && (long long)past + (end - tok0) <= (long long)a.width * LLMX_PAGE)))
+    n_new = end - tok0;
+  else if (threadIdx.x == 0)
+    llmx_report(20);
 }
 
 #define SAT_WS_ROW(D) ((D) + 4)        // a partial: numbers [D], max, sum, two unused (rows stay 16-byte aligned)
@@ -130,12 +142,12 @@ static int sat_refuse(const SatArgs& a, int fmt, int f32, int max_split) {
 }
 static SatArgs sat_args(const void* q, void* out, const void* k, const void* v, const float* ks, const float* vs, long long n_pages,
                         const int* table, int width, const int* seq_start, const int* seq_past, float* ws, int H, int G, int D,
-                        int window, int keep_first, int mask_chunk, float scale, int n_split, int max_rows, int settled) {
+                        int window, int keep_first, int mask_chunk, float scale, int n_split, int n_tokens, int max_new, int settled) {
   SatArgs a;
   a.q = q, a.out = out, a.k = (const uint8_t*)k, a.v = (const uint8_t*)v, a.ks = ks, a.vs = vs, a.table = table, a.seq_start = seq_start;
   a.seq_past = seq_past, a.ws = ws, a.width = width, a.n_pages = n_pages > 0x7fffffff ? 0 : (int)n_pages, a.H = H, a.G = G, a.D = D;
   a.window = window, a.keep_first = window > 0 ? keep_first : 0, a.mask_chunk = mask_chunk, a.n_split = n_split, a.tensor_copies = 0;
-  a.max_rows = max_rows, a.settled = settled, a.scale_log2 = scale * LLMX_LOG2E;
+  a.n_tokens = n_tokens, a.max_new = max_new, a.max_rows = G > 0 ? max_new * (H / G) : 0, a.settled = settled, a.scale_log2 = scale * LLMX_LOG2E;
   return a;
 }
 

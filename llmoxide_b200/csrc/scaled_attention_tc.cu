@@ -134,12 +134,13 @@ __global__ void __launch_bounds__(STC_THREADS, 1) scaled_chunk_tc_kernel(const S
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.z, H = a.H, G = a.G, R = H / G;
   const int g = blockIdx.x / a.n_split, share = blockIdx.x % a.n_split;
-  const int tok0 = a.seq_start[b], n_rows = (a.seq_start[b + 1] - tok0) * R;
+  int tok0, n_new, past;
+  sat_tokens(a, b, tok0, n_new, past);
+  const int n_rows = n_new * R;
   // heads and shares run fastest in launch order, and row tiles from the last one down: the longest walks start first
   const int row0 = (gridDim.y - 1 - blockIdx.y) * STC_ROWS;
   if (row0 >= n_rows) return;                         // uniform over the CTA, before anything is set up
   const int rows_here = min(STC_ROWS, n_rows - row0), n_x = rows_here > 128 ? 2 : 1;
-  const int past = a.seq_past[b];
   const int pos_lo = past + row0 / R, pos_hi = past + (row0 + rows_here - 1) / R;
   int first_lo = (a.window > 0 && pos_lo - (a.window - 1) > 0) ? pos_lo - (a.window - 1) : 0;
   if (a.mask_chunk > 0) first_lo = max(first_lo, pos_lo - pos_lo % a.mask_chunk);
@@ -556,7 +557,7 @@ LLMX_API int llmx_scaled_attention_chunk_tc(const void* q, void* out, const void
   if (B <= 0 || T <= 0 || max_new <= 0) return 0;
   if (G <= 0 || H <= 0 || (long long)max_new * (H / G) > 0x7fffffff - STC_ROWS) return LLMX_REFUSED(3);
   const SatArgs a = sat_args(q, out, k, v, k_scale, v_scale, n_pages, block_table, table_width, seq_start, seq_past, ws, H, G, D, window,
-                             keep_first, mask_chunk, scale, n_split, max_new * (H / G), 0);
+                             keep_first, mask_chunk, scale, n_split, T, max_new, 0);
   if (int code = sat_refuse(a, fmt, 0, STC_MAX_SPLIT)) return code;
   if ((D != 64 && D != 128) || !(scale > 0.f) || (n_split > 1 && !ws) || (((uintptr_t)q | (uintptr_t)out) & 15)) return LLMX_REFUSED(1);
   if (B > 65535 || (a.max_rows + STC_ROWS - 1) / STC_ROWS > 65535) return LLMX_REFUSED(3);

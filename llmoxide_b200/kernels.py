@@ -165,9 +165,11 @@ _STATUS_MEANING = {
                      2: "a token's sequence, position or page lies outside the launch's arrays (rows read)"},
     "scaled_attention": {1: "a copy into shared memory never completed",
                          2: "a visible key's page lies outside the launch's arrays",
-                         3: "its shared memory is not 1024-byte aligned"},
+                         3: "its shared memory is not 1024-byte aligned",
+                         20: "a sequence's tokens or positions lie outside the launch's arrays"},
     "scaled_attention_tc": {2: "a visible key's page lies outside the launch's arrays",
-                            3: "its shared memory is not 1024-byte aligned"},
+                            3: "its shared memory is not 1024-byte aligned",
+                            20: "a sequence's tokens or positions lie outside the launch's arrays"},
 }
 for _tiled in ("attention_prefill_tc", "attention_decode"):
     _STATUS_MEANING[_tiled + "_capped"] = _STATUS_MEANING[_tiled + "_biased"] = _STATUS_MEANING[_tiled]
@@ -1308,7 +1310,8 @@ def scaled_attention_chunk(q, out, k_cache, v_cache, k_scale, v_scale, block_tab
                            keep_first: int = 0, chunk: int = 0, n_shares: int = 0, tc=None) -> None:
     """Attention of several new tokens per sequence over a cache of 8-bit rows that holds them already: q, out [T,H*D] of
     bfloat16 or float32, packed sequence after sequence from ``seq_start`` [n_seqs+1]; ``seq_past[b]`` is the position of
-    sequence b's first new token, ``max_new`` the most of a sequence.  Masks and ``n_shares`` as in
+    sequence b's first new token, ``max_new`` the most of a sequence.  A sequence whose tokens or positions lie outside these
+    arrays is reported (``check_status``) and has no result.  Masks and ``n_shares`` as in
     ``scaled_attention_decode``.  ``tc`` (tests): the tcgen05 kernel or the other one; None: chosen."""
     fmt = _scaled_cache(k_cache, v_cache, k_scale, v_scale, block_table, n_kv_heads, head_dim)
     f32 = _scaled_attention(q, out, n_heads, n_kv_heads, head_dim, keep_first, chunk)

@@ -152,3 +152,38 @@ def test_a_loud_row_that_nobody_weighs(D, fmt):
                 out = torch.empty_like(q)
                 call(q, out, c, pos, H, shares)
                 check(out.view(1, H, D), out64, mag, score, largest * (8 if name == "tcgen05" else 1), dtype, L)
+
+
+@pytest.mark.parametrize("dtype, tc", [(torch.bfloat16, False), (torch.bfloat16, True), (torch.float32, False)])
+@pytest.mark.parametrize("shares", [1, 3])
+def test_sequences_outside_the_arrays_are_reported(dtype, tc, shares):
+    """Starts past the queries, in no order or negative, more tokens than ``max_new`` says, positions before 0 or past the block
+    table: nothing outside the arrays is read or written, the other sequence is right, and the host hears of it."""
+    from llmoxide_b200.errors import KernelError
+    H, G, D = 4, 2, 64
+    c = Cache([100, 70], G, D, "int8").fill()
+    T, n = 60, 30
+    q = torch.randn(T, H * D, generator=torch.Generator(DEV).manual_seed(6), device=DEV).to(dtype)
+    want = attend(q[:n].double().view(n, H, D), c.K[0], c.V[0], torch.arange(70, 100, device=DEV), None, 0, 0, D ** -0.5)
+    library = "scaled_attention_tc" if tc else "scaled_attention"
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    for start, past, max_new in (([0, n, T + 1], [70, 39], n + 1), ([0, n, 1 << 30], [70, 0], n), ([0, n, n - 5], [70, 40], n),
+                                 ([0, n, -7], [70, 40], n), ([0, n, T], [70, -1], n), ([0, n, T], [70, 99], n),
+                                 ([0, n, T], [70, (1 << 31) - 8], n), ([0, n, T], [70, -(1 << 31)], n)):
+        store = torch.full((T + 64, H * D), 7.0, dtype=dtype, device=DEV)
+        kernels().scaled_attention_chunk(q, store[:T], *c.args(), ints(start), ints(past), 2, max_new, H, G, D, None, D ** -0.5,
+                                         n_shares=shares, tc=tc)
+        torch.cuda.synchronize()
+        with pytest.raises(KernelError, match=library + ": a sequence's tokens or positions"):
+            kernels().check_status()
+        check(store[:n].view(n, H, D), *want, dtype, 100)
+        assert (store[T:] == 7.0).all()
+    # more tokens than max_new says
+    out = torch.full_like(q, 7.0)
+    kernels().scaled_attention_chunk(q, out, *c.args(), ints([0, n, T]), ints([70, 40]), 2, n - 1, H, G, D, None, D ** -0.5, n_shares=shares, tc=tc)
+    torch.cuda.synchronize()
+    with pytest.raises(KernelError, match="a sequence's tokens or positions"):
+        kernels().check_status()
+    kernels().scaled_attention_chunk(q, out, *c.args(), ints([0, n, T]), ints([70, 40]), 2, n, H, G, D, None, D ** -0.5, n_shares=shares, tc=tc)
+    kernels().check_status()
+    check(out[:n].view(n, H, D), *want, dtype, 100)
