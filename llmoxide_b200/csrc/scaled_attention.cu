@@ -119,7 +119,11 @@ scaled_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   const int sg = DP == 64 ? (gq & 4) | ((gq & 1) << 1) | ((gq >> 1) & 1) : gq;
   const int v0 = DP == 64 ? ((2 * tq) & 4) | (((2 * tq) >> 1) & 1) : 2 * tq, v1 = DP == 64 ? v0 + 2 : v0 + 1;
 
-  const int p = a.seq_past[b];
+  int p = a.seq_past[b];
+  if (p >= 0 && p / LLMX_PAGE >= a.width) {         // a position that the block table does not reach: no walk of millions of pages
+    if (threadIdx.x == 0) llmx_report(2);
+    p = -1;
+  }
   int first = (a.window > 0 && p - (a.window - 1) > 0) ? p - (a.window - 1) : 0;
   if (a.mask_chunk > 0 && p >= 0) first = max(first, p - p % a.mask_chunk);
   const int* pages = a.table + (size_t)b * a.width;

@@ -1261,7 +1261,8 @@ def scaled_attention_decode(q, out, k_cache, v_cache, k_scale, v_scale, block_ta
                             head_dim: int, window, scale: float, keep_first: int = 0, chunk: int = 0, n_shares: int = 0,
                             settled: bool = False) -> None:
     """``attention_decode`` over a cache of 8-bit rows: one new token per sequence, q, out [B,H*D] of bfloat16 or float32;
-    seq_past[b] is the token's position (-1: a sequence without keys, whose result is zeros).  ``window``, ``keep_first`` and
+    seq_past[b] is the token's position (-1: a sequence without keys, whose result is zeros; one past the block table is
+    reported).  ``window``, ``keep_first`` and
     ``chunk`` are the masks of ``attention_paged``.  ``n_shares`` (0: chosen from the batch's shape): into how many shares a
     sequence's keys are cut.  ``settled``: whatever wrote the block table, the positions and the rows before the new tokens'
     own has ended, so that those rows may be read while the launch before this one still runs (true of a step's attention,

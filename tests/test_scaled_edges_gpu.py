@@ -187,3 +187,22 @@ def test_sequences_outside_the_arrays_are_reported(dtype, tc, shares):
     kernels().scaled_attention_chunk(q, out, *c.args(), ints([0, n, T]), ints([70, 40]), 2, n, H, G, D, None, D ** -0.5, n_shares=shares, tc=tc)
     kernels().check_status()
     check(out[:n].view(n, H, D), *want, dtype, 100)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shares", [1, 3, 12])
+def test_a_position_past_the_block_table_is_reported(dtype, shares):
+    """A single token's: no key is walked to, and the other sequence is right."""
+    from llmoxide_b200.errors import KernelError
+    H, G, D = 4, 2, 64
+    c = Cache([100, 70], G, D, "int8").fill()
+    q = torch.randn(2, H * D, generator=torch.Generator(DEV).manual_seed(6), device=DEV).to(dtype)
+    for past in (128, 1 << 20, (1 << 31) - 1):
+        pos = torch.tensor([99, past], dtype=torch.int32, device=DEV)
+        out = torch.full_like(q, 7.0)
+        kernels().scaled_attention_decode(q, out, *c.args(), pos, H, G, D, None, D ** -0.5, n_shares=shares)
+        torch.cuda.synchronize()
+        with pytest.raises(KernelError, match="scaled_attention: a visible key's page"):
+            kernels().check_status()
+        check(out[:1].view(1, H, D), *attend(q[:1].double().view(1, H, D), c.K[0], c.V[0], pos[:1], None, 0, 0, D ** -0.5), dtype, 100)
+        assert (out[1] == 0).all()
