@@ -9,7 +9,8 @@
 // weight (scaled_rows.cuh), are rounded once to float16: 2^-12 of each, where the result's rounding to bfloat16 is 2^-9 on average.  float32 queries and weights go through the tensor cores as
 // two float16 terms, 22 bits.  Scores, maxima, sums and accumulators are float32.  A token that sees no key gets zeros.
 //
-// A hidden key's scale is never multiplied: it may be anything (a page's former owner, or a NaN row outside the window).
+// A hidden key's scale is never multiplied: it may be anything (a page's former owner, or a NaN row outside the window).  Nor do
+// the bytes past a sequence's last row count: e4m3 has codes for NaN, which a weight of 0 would not take away.
 #include "scaled_attention.cuh"
 
 __device__ __forceinline__ void sat_cp_async16(uint32_t dst, const void* src) {
@@ -280,6 +281,13 @@ scaled_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
           }
         }
 
+      if (FMT == ROWS_E4M3 && key0 + SAD_TILE - 1 > p) {              // the walk's last page: nothing is copied over it
+        for (int i = lane; i < SAD_TILE * (DP / 16); i += 32) {
+          const int r = i / (DP / 16);
+          if (key0 + r > p) *reinterpret_cast<uint4*>(smem + stage * S::STAGE + S::TILE + sat_at<DP, SAD_KEYS>(part + r, i % (DP / 16))) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        __syncwarp();
+      }
       const bool edge = key0 + SAD_TILE - 1 > p || key0 < first;      // some key of the tile is hidden
       float vscale[NI][2], vlog[NI][2];
 #pragma unroll
@@ -675,6 +683,13 @@ __global__ void __launch_bounds__(SAC_WARPS * 32) scaled_chunk_kernel(const SatA
     asm volatile("cp.async.wait_group 1;" ::: "memory");
     __syncthreads();
     const int key0 = tile_at(lo + t) * SAC_KEYS;
+    if (FMT == ROWS_E4M3 && key0 + SAC_KEYS - 1 > pos_hi) {           // the last page of the CTA's walk
+      for (int i = threadIdx.x; i < SAC_KEYS * pieces; i += SAC_WARPS * 32) {
+        const int r = i / pieces;
+        if (key0 + r > pos_hi) *reinterpret_cast<uint4*>(smem + stage * S::STAGE + S::TILE + sat_at<DP, SAC_KEYS>(r, i % pieces)) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      __syncthreads();
+    }
     const uint32_t sK = base + stage * S::STAGE, sV = sK + S::TILE, sS = base + S::SCALES + stage * 2 * SAC_KEYS * 4;
     float s[8][4];                                  // rows gq and gq + 8, keys 8 i + 2 tq and + 1
 #pragma unroll

@@ -105,14 +105,20 @@ __device__ __forceinline__ void stc_bulk(uint32_t dst, const void* src, uint32_t
 }
 
 // A page of 8-bit rows as a float16 tile, by 128 threads: a thread takes 16 bytes of a row, which are two pieces of a
-// panel's 128-byte row.  (Threads of the second half of a row write theirs in the other order: no bank conflicts.)
+// panel's 128-byte row.  (Threads of the second half of a row write theirs in the other order: no bank conflicts.)  Rows from
+// `live` on become zeros.
 template <int D, int FMT>
-__device__ __forceinline__ void stc_convert(uint8_t* smem, int raw, int tile, int t) {
+__device__ __forceinline__ void stc_convert(uint8_t* smem, int raw, int tile, int t, int live) {
   constexpr int C = D / 16, STEP = 128 / C;          // pieces of a row; rows at a time
   const int c = t % C;
   uint4 x[STC_KEYS / STEP];
 #pragma unroll
   for (int i = 0; i < STC_KEYS / STEP; ++i) x[i] = *reinterpret_cast<const uint4*>(smem + raw + (t / C + i * STEP) * D + c * 16);
+  if (live < STC_KEYS) {
+#pragma unroll
+    for (int i = 0; i < STC_KEYS / STEP; ++i)
+      if (t / C + i * STEP >= live) x[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
 #pragma unroll
   for (int i = 0; i < STC_KEYS / STEP; ++i) {
     const int r = t / C + i * STEP;
@@ -267,7 +273,7 @@ __global__ void __launch_bounds__(STC_THREADS, 1) scaled_chunk_tc_kernel(const S
       for (int x = 0; x < n_x && j >= 2; ++x) wait(pair_bar(s_full, x, st), ((j >> 1) & 1) ^ 1, 10);
       if (__any_sync(0xffffffffu, gave_up)) break;
       tc_fence_after();
-      stc_convert<D, FMT>(smem, raw, S::K + st * S::TILE, t);
+      stc_convert<D, FMT>(smem, raw, S::K + st * S::TILE, t, STC_KEYS);
       if (warp == 4) {
         // the tile's scales: of hidden keys they may be anything, and count for nothing (those that only some rows see are
         // left to the rows)
@@ -296,7 +302,7 @@ __global__ void __launch_bounds__(STC_THREADS, 1) scaled_chunk_tc_kernel(const S
       if (lane == 0) mbar_arrive(k_ready + 8 * st);
       for (int x = 0; x < n_x && j >= 2; ++x) wait(pair_bar(pv_done, x, st), ((j >> 1) & 1) ^ 1, 11);
       tc_fence_after();
-      stc_convert<D, FMT>(smem, raw + S::RAW, S::V + st * S::TILE, t);
+      stc_convert<D, FMT>(smem, raw + S::RAW, S::V + st * S::TILE, t, FMT == ROWS_E4M3 ? pos_hi + 1 - key0 : STC_KEYS);      // (NaN codes past the end)
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) {

@@ -206,3 +206,37 @@ def test_a_position_past_the_block_table_is_reported(dtype, shares):
             kernels().check_status()
         check(out[:1].view(1, H, D), *attend(q[:1].double().view(1, H, D), c.K[0], c.V[0], pos[:1], None, 0, 0, D ** -0.5), dtype, 100)
         assert (out[1] == 0).all()
+
+
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+def test_what_lies_past_a_sequences_end_is_nobodys(D):
+    """Pages that no writer has touched past a sequence's last row, here all bits set: NaN codes in e4m3, under NaN scales."""
+    H, G = 4, 2
+    past, new = [64, 0, 90, 129], [30, 5, 1, 64]
+    for fmt in FMT:
+        c = Cache([p + n for p, n in zip(past, new)], G, D, fmt).fill()
+        for b, n in enumerate(c.lengths):
+            page, row = int(c.table[b, (n - 1) // PAGE]), (n - 1) % PAGE + 1
+            for store in (c.k, c.v):
+                store.view(torch.int8)[page, :, row:] = -1
+        ints = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+        start, T = [sum(new[:i]) for i in range(len(new) + 1)], sum(new)
+        for dtype in (torch.bfloat16, torch.float32):
+            q = torch.randn(T, H * D, generator=torch.Generator(DEV).manual_seed(7), device=DEV).to(dtype)
+            want = [attend(q[start[b] : start[b] + n].double().view(n, H, D), c.K[b], c.V[b], torch.arange(p, p + n, device=DEV), None, 0, 0,
+                           D ** -0.5) for b, (p, n) in enumerate(zip(past, new))]
+            for tc in (False, True) if dtype == torch.bfloat16 and D in (64, 128) else (False,):
+                for shares in (1, 3):
+                    out = torch.empty_like(q)
+                    kernels().scaled_attention_chunk(q, out, *c.args(), ints(start), ints(past), len(new), max(new), H, G, D, None, D ** -0.5,
+                                                     n_shares=shares, tc=tc)
+                    for b, n in enumerate(new):
+                        check(out[start[b] : start[b] + n].view(n, H, D), *want[b], dtype, past[b] + n)
+            last = torch.tensor(start[1:], device=DEV) - 1
+            for shares in (1, 3):
+                out = torch.empty(len(new), H * D, dtype=dtype, device=DEV)
+                kernels().scaled_attention_decode(q[last], out, *c.args(), ints([n - 1 for n in c.lengths]), H, G, D, None, D ** -0.5,
+                                                  n_shares=shares)
+                for b in range(len(new)):
+                    check(out[b].view(1, H, D), *(x[-1:] for x in want[b]), dtype, c.lengths[b])
+    kernels().check_status()
