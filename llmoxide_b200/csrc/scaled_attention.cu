@@ -518,7 +518,7 @@ static int launch_decode(SatArgs a, int B, cudaStream_t stream) {
     launch_pdl(kernel, grid, dim3(SAD_THREADS), smem, stream, mk, mv, a);
   const int code = LLMX_LAUNCH_STATUS();
   if (code || a.n_split <= SAD_CLUSTER) return code;
-  return launch_merge<TERMS>(a, (long long)B * a.H, stream);
+  return launch_merge<TERMS>(a, (long long)B * a.H, B, stream);
 }
 template <int DP, int FMT>
 static int launch_decode_by_type(const SatArgs& a, int B, int f32, cudaStream_t stream) {
@@ -847,7 +847,7 @@ static int launch_chunk(const SatArgs& a, int B, long long T, cudaStream_t strea
   launch_pdl(kernel, dim3((a.max_rows + SAC_ROWS - 1) / SAC_ROWS, a.G * a.n_split, B), dim3(SAC_WARPS * 32), smem, stream, a);
   const int code = LLMX_LAUNCH_STATUS();
   if (code || a.n_split == 1) return code;
-  return launch_merge<TERMS>(a, T * a.H, stream);
+  return launch_merge<TERMS>(a, T * a.H, B, stream);
 }
 
 // q, out: [T, H*D], tokens packed sequence after sequence (seq_start [B+1]); seq_past[b]: position of the first of them; max_new:

@@ -68,9 +68,11 @@ __device__ __forceinline__ void sat_store4(void* out, size_t at, float4 v) {
 
 // Partials [rows][n_split][D + 4] = (numbers, max, sum) -> out [rows][D]: WARPS warps a row, every WARPS-th share each, several
 // asked for together.  Four warps where rows are few and shares many (a decode step of 32 rows of 40 shares: 27 us with its
-// attention, 33 by one warp a row), one elsewhere (128 tokens' 4096 rows of nine shares: 36 us with theirs, 46 by four).
+// attention, 33 by one warp a row), one elsewhere (128 tokens' 4096 rows of nine shares: 36 us with theirs, 46 by four).  With
+// seq_start [n_seqs + 1], rows of tokens that belong to no sequence have no partials, and are left alone.
 template <int TERMS, int WARPS>
-__global__ void __launch_bounds__(128) scaled_merge_kernel(const float* __restrict__ ws, void* out, long long rows, int n_split, int D) {
+__global__ void __launch_bounds__(128) scaled_merge_kernel(const float* __restrict__ ws, void* out, long long rows, int n_split, int D,
+                                                           const int* __restrict__ seq_start, int n_seqs, int H) {
   __shared__ float4 part[WARPS > 1 ? WARPS : 1][WARPS > 1 ? 64 : 1];
   __shared__ float sums[WARPS];
   pdl_launch_dependents();
@@ -79,12 +81,24 @@ __global__ void __launch_bounds__(128) scaled_merge_kernel(const float* __restri
   const long long row = (long long)blockIdx.x * (4 / WARPS) + warp / WARPS;
   if (row >= rows) return;                          // (with four warps a row, the whole CTA)
   const float* base = ws + (size_t)row * n_split * SAT_WS_ROW(D);
+  const int start = seq_start && lane <= n_seqs ? __ldg(seq_start + lane) : 0;      // (asked for here, looked at where it has come)
   float mx = -INFINITY;
   for (int c = lane; c < n_split; c += 32) mx = fmaxf(mx, __ldcg(base + (size_t)c * SAT_WS_ROW(D) + D));
   mx = warp_max(mx);
+  // The largest end counts: a sequence out of order is reported, the others have results.
+  auto of_a_sequence = [&]() {
+    if (!seq_start) return true;
+    int end = start;
+    for (int i = lane + 32; i <= n_seqs; i += 32) end = max(end, __ldg(seq_start + i));
+    return row >= (long long)__shfl_sync(0xffffffffu, start, 0) * H && __any_sync(0xffffffffu, row < (long long)end * H);
+  };
   float ls = 0.f;
-  for (int d = 4 * lane; d < D; d += 128) {
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 acc[2];                                    // dims 4 lane .. and 128 + 4 lane ..
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int d = 4 * lane + 128 * i;
+    acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (d >= D) continue;
     ls = 0.f;
 #pragma unroll(WARPS > 1 ? 8 : 4)
     for (int c = mine; c < n_split; c += WARPS) {
@@ -93,17 +107,23 @@ __global__ void __launch_bounds__(128) scaled_merge_kernel(const float* __restri
       const float4 v = __ldcg(reinterpret_cast<const float4*>(src + d));
       if (ml.y == 0.f) continue;                    // a share that got no key
       const float f = exp2f(ml.x - mx);
-      acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+      acc[i].x += f * v.x, acc[i].y += f * v.y, acc[i].z += f * v.z, acc[i].w += f * v.w;
       ls += f * ml.y;
     }
-    if (WARPS > 1) {
-      part[mine][d / 4] = acc;
-    } else {
-      const float r = ls == 0.f ? 0.f : 1.f / ls;
-      sat_store4<TERMS>(out, (size_t)row * D + d, make_float4(acc.x * r, acc.y * r, acc.z * r, acc.w * r));
-    }
   }
-  if (WARPS == 1) return;
+  if (!of_a_sequence()) return;                     // (all of the row's warps)
+  if (WARPS == 1) {
+    const float r = ls == 0.f ? 0.f : 1.f / ls;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int d = 4 * lane + 128 * i;
+      if (d < D) sat_store4<TERMS>(out, (size_t)row * D + d, make_float4(acc[i].x * r, acc[i].y * r, acc[i].z * r, acc[i].w * r));
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (4 * lane + 128 * i < D) part[mine][lane + 32 * i] = acc[i];
   if (lane == 0) sums[mine] = ls;                   // (lane 0 has dims of its own at every size)
   __syncthreads();
   for (int i = threadIdx.x; i < D / 4; i += 128) {
@@ -120,12 +140,14 @@ __global__ void __launch_bounds__(128) scaled_merge_kernel(const float* __restri
   }
 }
 template <int TERMS>
-static int launch_merge(const SatArgs& a, long long rows, cudaStream_t stream) {
+static int launch_merge(const SatArgs& a, long long rows, int n_seqs, cudaStream_t stream) {
   if (rows > 0x7fffffffll) return LLMX_REFUSED(3);
   if (a.n_split > 8 && rows <= 256)
-    launch_pdl(scaled_merge_kernel<TERMS, 4>, dim3((unsigned)rows), dim3(128), 0, stream, (const float*)a.ws, a.out, rows, a.n_split, a.D);
+    launch_pdl(scaled_merge_kernel<TERMS, 4>, dim3((unsigned)rows), dim3(128), 0, stream, (const float*)a.ws, a.out, rows, a.n_split, a.D,
+               a.seq_start, n_seqs, a.H);
   else
-    launch_pdl(scaled_merge_kernel<TERMS, 1>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, stream, (const float*)a.ws, a.out, rows, a.n_split, a.D);
+    launch_pdl(scaled_merge_kernel<TERMS, 1>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, stream, (const float*)a.ws, a.out, rows, a.n_split, a.D,
+               a.seq_start, n_seqs, a.H);
   return LLMX_LAUNCH_STATUS();
 }
 

@@ -551,7 +551,7 @@ static int launch_chunk_tc(const SatArgs& a, int B, long long T, cudaStream_t st
   launch_pdl(kernel, dim3(a.G * a.n_split, (a.max_rows + STC_ROWS - 1) / STC_ROWS, B), dim3(STC_THREADS), smem, stream, a);
   const int code = LLMX_LAUNCH_STATUS();
   if (code || a.n_split == 1) return code;
-  return launch_merge<1>(a, T * a.H, stream);
+  return launch_merge<1>(a, T * a.H, B, stream);
 }
 
 // As llmx_scaled_attention_chunk, for bfloat16, D 64 or 128 and scale > 0.

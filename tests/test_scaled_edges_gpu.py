@@ -240,3 +240,22 @@ def test_what_lies_past_a_sequences_end_is_nobodys(D):
                 for b in range(len(new)):
                     check(out[b].view(1, H, D), *(x[-1:] for x in want[b]), dtype, c.lengths[b])
     kernels().check_status()
+
+
+@pytest.mark.parametrize("dtype, tc", [(torch.bfloat16, False), (torch.bfloat16, True), (torch.float32, False)])
+def test_rows_of_no_sequence_are_left_alone(dtype, tc):
+    """Queries before the first sequence's and behind the last one's, as a padded step has them, in one share or several."""
+    H, G, D = 4, 2, 64
+    c = Cache([700, 70], G, D, "int8").fill()
+    T, lo, mid, hi = 40, 3, 13, 20
+    q = torch.randn(T, H * D, generator=torch.Generator(DEV).manual_seed(6), device=DEV).to(dtype)
+    start, past = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([lo, mid, hi], [690, 63]))
+    for shares in (1, 3, 11):
+        out = torch.full_like(q, 7.0)
+        kernels().scaled_attention_chunk(q, out, *c.args(), start, past, 2, 10, H, G, D, None, D ** -0.5, n_shares=shares, tc=tc)
+        assert (out[:lo] == 7.0).all() and (out[hi:] == 7.0).all()
+        for b, rows in enumerate((slice(lo, mid), slice(mid, hi))):
+            n = rows.stop - rows.start
+            at = int(past[b]) + torch.arange(n, device=DEV)
+            check(out[rows].view(n, H, D), *attend(q[rows].double().view(n, H, D), c.K[b], c.V[b], at, None, 0, 0, D ** -0.5), dtype, c.lengths[b])
+    kernels().check_status()
