@@ -1313,7 +1313,7 @@ def scaled_attention_chunk(q, out, k_cache, v_cache, k_scale, v_scale, block_tab
     bfloat16 or float32, packed sequence after sequence from ``seq_start`` [n_seqs+1]; ``seq_past[b]`` is the position of
     sequence b's first new token, ``max_new`` the most of a sequence.  A sequence whose tokens or positions lie outside these
     arrays is reported (``check_status``) and has no result; tokens of no sequence are left alone.  Masks and ``n_shares`` as in
-    ``scaled_attention_decode``.  ``tc`` (tests): the tcgen05 kernel or the other one; None: chosen."""
+    ``scaled_attention_decode``.  ``tc``: the tcgen05 kernel or the other one (mma.sync); None: chosen."""
     fmt = _scaled_cache(k_cache, v_cache, k_scale, v_scale, block_table, n_kv_heads, head_dim)
     f32 = _scaled_attention(q, out, n_heads, n_kv_heads, head_dim, keep_first, chunk)
     T, rows = q.shape[0], max(1, max_new) * (n_heads // n_kv_heads)

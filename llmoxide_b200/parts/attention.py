@@ -260,7 +260,8 @@ class GQAttention:
         if self.keys_as_values:
             libs.add("qk_unit")
         if self.rows is not None:
-            return libs | {"scaled_cache", "scaled_attention", "scaled_attention_tc"}
+            tc = self.rt.tensor_cores and self.rt.act_dtype == torch.bfloat16 and self.D in (64, 128) and self.scale > 0
+            return libs | {"scaled_cache", "scaled_attention"} | ({"scaled_attention_tc"} if tc else set())
         if not self.plain:
             return libs | {"attention"}
         if self.rt.dtype == "bfloat16" and self.rt.tensor_cores:
@@ -347,7 +348,7 @@ class GQAttention:
         return self.o(out, splits_ok=True, add_bias=not self.defer_out_bias)
 
     def attend(self, q, out, view, block_table, ctx):
-        """8-bit rows: the kernel of single tokens, or of several.  Otherwise, bfloat16: the split-key kernel when every sequence brings one token;
+        """8-bit rows: the kernel of single tokens, or of several (on tcgen05 where the runtime wants that).  Otherwise, bfloat16: the split-key kernel when every sequence brings one token;
         for prompts the tcgen05 kernel at head size 128 and the mma.sync tiled
         kernel at head size 64; the general kernel otherwise (values of another
         size than the keys among them) and always in float32.  All of them take
@@ -360,7 +361,8 @@ class GQAttention:
                                                 keep_first=self.keep_first, chunk=self.chunk, settled=True)
             else:
                 kernels.scaled_attention_chunk(q, out, *cache, ctx.seq_start, ctx.seq_past, ctx.n_seqs, ctx.max_new, H, G, D,
-                                               self.window, self.scale, keep_first=self.keep_first, chunk=self.chunk)
+                                               self.window, self.scale, keep_first=self.keep_first, chunk=self.chunk,
+                                               tc=None if self.rt.tensor_cores else False)
             return
         fast = (self.plain and q.dtype == torch.bfloat16 and view.k.dtype == torch.bfloat16
                 and self.rt.tensor_cores and self.scale > 0)       # (the tiled kernels take the maximum before the scale)

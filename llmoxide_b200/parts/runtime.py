@@ -17,7 +17,7 @@ class Runtime:
     dtype: str                 # "bfloat16" (serving precisions) or "float32" (true 32-bit everywhere)
     device: torch.device
     max_positions: int         # longest sequence the cache allows; sizes position tables
-    tensor_cores: bool = True  # bfloat16 only: use the tcgen05 matrix product where it applies
+    tensor_cores: bool = True  # bfloat16 only: use the tcgen05 kernels where they apply (attention over 8-bit rows: mma.sync otherwise)
     shared: dict = field(default_factory=dict)  # objects that parts of one model share (position tables)
     # what keys and values are cached as: None as the activations, or 8-bit rows with a scale each (see ROW_DTYPES)
     row_dtype: Optional[torch.dtype] = None

@@ -259,3 +259,29 @@ def test_rows_of_no_sequence_are_left_alone(dtype, tc):
             at = int(past[b]) + torch.arange(n, device=DEV)
             check(out[rows].view(n, H, D), *attend(q[rows].double().view(n, H, D), c.K[b], c.V[b], at, None, 0, 0, D ** -0.5), dtype, c.lengths[b])
     kernels().check_status()
+
+
+@pytest.mark.parametrize("name", ["D", "E"])
+def test_an_engine_without_tcgen05(tmp_path, monkeypatch, name):
+    """``tensor_cores=False``: prompts over 8-bit rows go by the other kernel, and the tcgen05 one is not even loaded.  Bound: as in
+    test_scaled_engine_gpu.py, the wide cache's tolerance and twice what rounding the cache does."""
+    import numpy as np
+    from replay_util import TOL
+    from test_scaled_engine_gpu import folder_of, load
+    from tiny_configs import ALL
+    folder = folder_of(tmp_path, name, "bfloat16")
+    toks = np.random.default_rng(3).integers(0, ALL[name]["vocab_size"], 150).tolist()
+    called, find = [], kernels()._scaled_fn
+    monkeypatch.setattr(kernels(), "_scaled_fn", lambda key: (called.append(key), find(key))[1])
+    logits, by = [], []
+    for fmt, tensor_cores in (("", True), ("int8", True), ("int8", False)):
+        eng = load(folder, "bfloat16", fmt, tensor_cores=tensor_cores)
+        del called[:]
+        slot = eng.acquire()
+        logits.append(torch.cat([eng.step([(slot, toks[:149])], [list(range(149))]), eng.step([(slot, toks[149:])])]).double())
+        eng.check_status()
+        by.append((set(lib for lib, _ in called), eng.model.libraries()))
+    assert "scaled_attention_tc" in by[1][0] and "scaled_attention_tc" in by[1][1]
+    assert "scaled_attention_tc" not in by[2][0] and "scaled_attention_tc" not in by[2][1] and "scaled_attention" in by[2][0]
+    off = lambda a, b: float((logits[a] - logits[b]).abs().max() / logits[0].abs().max())
+    assert off(1, 2) <= TOL["bfloat16"] + 2 * off(0, 1)
