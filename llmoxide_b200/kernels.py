@@ -1284,10 +1284,10 @@ def scaled_attention_decode(q, out, k_cache, v_cache, k_scale, v_scale, block_ta
              head_dim, window or 0, keep_first or 0, chunk or 0, scale, n, settled, _stream()), "scaled_attention_decode")
 
 
-def scaled_chunk_tc_supports(q, head_dim: int, scale: float) -> bool:
-    """Whether the tcgen05 kernel takes the product, which it does wherever it can.  (Two tokens of 8 sequences at 2000, 32
+def scaled_chunk_tc_supports(q, out, head_dim: int, scale: float) -> bool:
+    """Whether the tcgen05 kernel takes the product (queries and results by 16 bytes), which it does wherever it can.  (Two tokens of 8 sequences at 2000, 32
     heads over 8 of 128: 26 us, 37 with the other; of 16 sequences, 8 heads of 64: 34, 38 with the other.)"""
-    return q.dtype is torch.bfloat16 and scale > 0 and head_dim in (64, 128)
+    return q.dtype is torch.bfloat16 and scale > 0 and head_dim in (64, 128) and not (q.data_ptr() | out.data_ptr()) & 15
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1320,7 +1320,7 @@ def scaled_attention_chunk(q, out, k_cache, v_cache, k_scale, v_scale, block_tab
     _int32("seq_start", seq_start, 1, n_seqs + 1), _int32("seq_past", seq_past, 1, n_seqs)
     if block_table.shape[0] < n_seqs:
         raise KernelError(f"a block table of {block_table.shape[0]} rows for {n_seqs} sequences")
-    tc = scaled_chunk_tc_supports(q, head_dim, scale) if tc is None else tc
+    tc = scaled_chunk_tc_supports(q, out, head_dim, scale) if tc is None else tc
     n = n_shares or scaled_chunk_shares(max(1, n_seqs), n_kv_heads, rows,
                                         _mask_pages(block_table.shape[1], window, keep_first, chunk, max_new), tc, q.numel(), _sm_of(q))
     ws = guard.scratch((T * n_heads * n * (head_dim + 4),), torch.float32, q.device,

@@ -285,3 +285,24 @@ def test_an_engine_without_tcgen05(tmp_path, monkeypatch, name):
     assert "scaled_attention_tc" not in by[2][0] and "scaled_attention_tc" not in by[2][1] and "scaled_attention" in by[2][0]
     off = lambda a, b: float((logits[a] - logits[b]).abs().max() / logits[0].abs().max())
     assert off(1, 2) <= TOL["bfloat16"] + 2 * off(0, 1)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_queries_that_start_between_vectors(D):
+    """bfloat16 queries and results on 8-byte boundaries: the kernel of 16-byte loads does not take them, the other does."""
+    H, G, n = 4, 2, 20
+    c = Cache([100], G, D, "int8").fill()
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    base = torch.randn(n * H * D + 8, generator=torch.Generator(DEV).manual_seed(6), device=DEV).to(torch.bfloat16)
+    q = base[4 : 4 + n * H * D].view(n, H * D)
+    want = attend(q.double().view(n, H, D), c.K[0], c.V[0], torch.arange(80, 100, device=DEV), None, 0, 0, D ** -0.5)
+    for q_at, out_at in ((4, 0), (0, 4), (4, 4)):
+        x = base[:n * H * D].clone().view(n, H * D).copy_(q) if q_at == 0 else q
+        store = torch.full((n * H * D + 8,), 7.0, dtype=torch.bfloat16, device=DEV)
+        out = store[out_at : out_at + n * H * D].view(n, H * D)
+        kernels().scaled_attention_chunk(x, out, *c.args(), ints([0, n]), ints([80]), 1, n, H, G, D, None, D ** -0.5)
+        check(out.view(n, H, D), *want, torch.bfloat16, 100)
+        one = torch.empty(8 + H * D, dtype=torch.bfloat16, device=DEV)[out_at : out_at + H * D].view(1, H * D)
+        kernels().scaled_attention_decode(x[-1:], one, *c.args(), ints([99]), H, G, D, None, D ** -0.5)
+        check(one.view(1, H, D), *(y[-1:] for y in want), torch.bfloat16, 100)
+    kernels().check_status()
