@@ -1243,9 +1243,11 @@ def scaled_decode_shares(n_seqs: int, n_kv_heads: int, group: int, n_pages: int,
     8 that merge inside a thread-block cluster (64 tokens of 32 heads over 8 from depth 2048: 50 us in one share, 64 in
     four; 8 of them: 12.3 us in six, 20.8 in one), a CTA at least four pages.  Where the CTAs do not fit at once anyhow,
     shares of 32 pages or more, up to four, level the ends of unequal sequences (64 up to depth 16001: 279 us in one,
-    240 in four).  Beyond eight the partials go through a workspace and a second launch, which pays for long walks
-    (one sequence at depth 32768: 41 us in eight, 27 in 48; two: 45 and 30 in 32).  Not a CTA a multiprocessor, though they
-    would all fit: 136 to 152 of them take 37 us, some multiprocessors two while others have none."""
+    240 in four).  Beyond eight the partials go through a workspace and a second launch, which pays for long walks of one
+    sequence (depth 32768, 8 kv heads of 128: 45 us in eight, 26 in 48, which is taken from 192 pages and below 12 CTAs a share
+    on).  Two to eight sequences as deep stay with the cluster, though they would gain as well (two 49 us in eight, 29 in 32;
+    four 73 and 46 in 16; eight 99 in six, 74 in 16; heads of 64 alike); at depth 8192 they would hardly (two 19 and 17).  Not a CTA a
+    multiprocessor, though they would all fit: 136 to 152 of them take 37 us, some multiprocessors two while others have none."""
     heads = 16 if group > 8 and head_dim <= 128 and not f32 else 8
     base = n_seqs * n_kv_heads * ((group + heads - 1) // heads)
     resident = sms * (4 if head_dim <= 64 else 3 if head_dim <= 128 else 2)
