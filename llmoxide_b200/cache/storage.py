@@ -32,8 +32,8 @@ class KVNeed:
     values in a dtype of its own (default: the runtime's cache dtype).  With ``pool`` n > 1 the entry owns a second
     store beside the first, one key and one value per block of n positions (block b = positions b*n .. b*n+n-1, its
     row exists once the sequence holds all of them); that store keeps every row, whatever the window.  ``every`` is
-    how many positions one row of a store stands for (the second store's description; 1 for the first).  Keys and values
-    of an 8-bit ``dtype`` (int8, float8_e4m3fn) come with a float32 scale a row beside them."""
+    how many positions one row of a store stands for (the second store's description; 1 for the first).  ``scaled``: keys
+    and values have a float32 scale a row beside them (rows of int8 or float8_e4m3fn)."""
 
     n_kv_heads: int
     head_dim: int
@@ -43,10 +43,7 @@ class KVNeed:
     keep_first: int = 0
     pool: int = 0
     every: int = 1
-
-    @property
-    def scaled(self) -> bool:
-        return self.dtype in (torch.int8, torch.float8_e4m3fn)
+    scaled: bool = False
 
     def pooled(self) -> "KVNeed":
         """The description of the store of one row per block that goes with this entry."""

@@ -73,8 +73,7 @@ class Engine:
         self.rt = Runtime(dtype=options.dtype, device=self.device, max_positions=max_seq,
                           tensor_cores=options.tensor_cores, row_dtype=ROW_DTYPES.get(options.cache_dtype))
         self.model = DecoderModel(self.spec, weights, self.rt)
-        if self.rt.row_dtype is not None and any(kv is not None and kv.dtype != self.rt.row_dtype
-                                                 for kv, _ in self.model.cache_needs()):
+        if self.rt.row_dtype is not None and any(kv is not None and not kv.scaled for kv, _ in self.model.cache_needs()):
             raise Unsupported(f"cache_dtype {options.cache_dtype!r}: a layer of this model caches rows that are not built as 8-bit rows")
         # Every library the model will launch is built and made resident now, while the GPU is idle: a step
         # never has to stop for one.

@@ -242,7 +242,7 @@ class GQAttention:
     def cache_need(self):
         state = StateNeed((self.taps - 1, self.channels)) if self.taps > 1 else None
         return KVNeed(self.G, self.D, self.cache_window, v_head_dim=None if self.Dv == self.D else self.Dv,
-                      dtype=self.rows, keep_first=self.cache_keep_first, pool=self.pool), state
+                      dtype=self.rows, keep_first=self.cache_keep_first, pool=self.pool, scaled=self.rows is not None), state
 
     @property
     def takes_row_scales(self) -> bool:

@@ -25,3 +25,17 @@ def test_single_tokens_always_have_a_share_of_some_pages():
 def test_several_tokens(n_seqs, new, past, want):
     pages = (new + past + 63) // 64
     assert kernels.scaled_chunk_shares(n_seqs, 8, 4 * new, pages, True, n_seqs * new * 4096) == want
+
+
+def test_only_those_that_ask_get_scales():
+    """An entry whose own numbers are of 8 bits, as another kind of layer may keep them, is stored as it is."""
+    import torch
+
+    from llmoxide_b200.cache import Cache, PAGE
+    from llmoxide_b200.cache.storage import KVNeed
+    for dtype in (torch.int8, torch.float8_e4m3fn):
+        plain = Cache([(KVNeed(2, 32, dtype=dtype), None)], 1, 2 * PAGE, torch.float32, torch.device("cpu"))
+        assert plain.bytes() == 2 * 2 * PAGE * 2 * 32 and plain.view(0).k_scale is None and plain.view(0).v_scale is None
+        rows = Cache([(KVNeed(2, 32, dtype=dtype, scaled=True), None)], 1, 2 * PAGE, torch.float32, torch.device("cpu"))
+        assert rows.bytes() == 2 * 2 * PAGE * 2 * (32 + 4) and rows.view(0).k_scale.shape == rows.view(0).k.shape[:3]
+        rows.wipe(), plain.wipe()
