@@ -6,6 +6,13 @@
 
 template <int TERMS> __device__ __forceinline__ float sat_exp2(float x) { return TERMS == 1 ? ex2_approx(x) : exp2f(x); }
 
+// A stretch of memory into shared memory; its bytes are counted by a barrier.
+__device__ __forceinline__ void sat_bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
 // Four query numbers from dim d of a row.
 template <int TERMS>
 __device__ __forceinline__ float4 sat_query4(const void* q, size_t row, int d) {

@@ -98,11 +98,6 @@ __device__ __forceinline__ uint32_t stc_f16x2(float x, float y) {
   const __half2 h = __floats2half2_rn(x, y);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ void stc_bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
 
 // A page of 8-bit rows as a float16 tile, by 128 threads: a thread takes 16 bytes of a row, which are two pieces of a
 // panel's 128-byte row.  (Threads of the second half of a row write theirs in the other order: no bank conflicts.)  Rows from
@@ -209,10 +204,10 @@ __global__ void __launch_bounds__(STC_THREADS, 1) scaled_chunk_tc_kernel(const S
         const size_t row = ((size_t)sat_page(a, pages, key_at(j) / LLMX_PAGE) * G + g) * LLMX_PAGE;
         const uint32_t to = base + S::RAW0 + st * S::RAW_STAGE, bar = raw_full + 8 * st;
         mbar_expect_tx(bar, S::RAW_STAGE);
-        stc_bulk(to, a.k + row * D, S::RAW, bar);
-        stc_bulk(to + S::RAW, a.v + row * D, S::RAW, bar);
-        stc_bulk(to + 2 * S::RAW, a.ks + row, STC_KEYS * 4, bar);
-        stc_bulk(to + 2 * S::RAW + STC_KEYS * 4, a.vs + row, STC_KEYS * 4, bar);
+        sat_bulk(to, a.k + row * D, S::RAW, bar);
+        sat_bulk(to + S::RAW, a.v + row * D, S::RAW, bar);
+        sat_bulk(to + 2 * S::RAW, a.ks + row, STC_KEYS * 4, bar);
+        sat_bulk(to + 2 * S::RAW + STC_KEYS * 4, a.vs + row, STC_KEYS * 4, bar);
       }
       // no copy outlives the CTA, also where the others have given up
       for (int i = max(0, j - 2); i < j; ++i) mbar_wait(raw_full + 8 * (i & 1), (i >> 1) & 1);
