@@ -68,8 +68,8 @@ template <int DP> __device__ __forceinline__ int sat_piece(int u, int tq) { retu
 // side (16 of a key's row a load; of a value's row 16 dims for each of four keys, paired across keys by the byte
 // permutation that the conversion starts with).  No ldmatrix, no transposition.
 //
-// 64 sequences at up to 16000, 32 heads over 8 of 128, e4m3: 1.45 GB in 233 us, 6.2 TB/s, 0.95 of a copy's; 46 % of the issue slots.
-// Eight at 2048: 12.4 us, of which some 5 are the launch, the first trip to memory and the merge.
+// 64 sequences at up to 16000, 32 heads over 8 of 128, e4m3: 1.45 GB in 233 to 251 us by card, 5.8 to 6.2 TB/s,
+// 0.88 to 0.94 of a copy's; 44 % of the issue slots.  Eight at 2048: 12.7 us, of which some 5 are the launch, the first trip to memory and the merge.
 //
 // The shares of a (sequence, kv head, head group) are a thread-block cluster (up to 8) that merges its partials out of one
 // another's shared memory, or go through a workspace and a second kernel.  Sums run in share order.
@@ -552,7 +552,7 @@ LLMX_API int llmx_scaled_attention_decode(const void* q, void* out, int f32, con
 // (token, head of the kv head) pairs, token after token, so that a few tokens fill a tile with the heads that share their
 // keys; a CTA of four warps takes 64 of them, 16 a warp, and walks the visible keys a page of 64 at a time.  All four
 // warps convert every cached byte for 16 rows, which is what bounds it: 2048 tokens after 6144, 32 heads over 8 of 128, take
-// 1456 us (165 TFLOP/s) where the tcgen05 kernel, which converts once for 256 rows, takes 331.  With n_split > 1 the walk is cut into shares whose partials meet in scaled_merge_kernel.
+// 1570 us (154 TFLOP/s) where the tcgen05 kernel, which converts once for 256 rows, takes 341.  With n_split > 1 the walk is cut into shares whose partials meet in scaled_merge_kernel.
 // ---------------------------------------------------------------------------
 #define SAC_WARPS 4
 #define SAC_ROWS (16 * SAC_WARPS)

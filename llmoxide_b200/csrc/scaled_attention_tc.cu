@@ -20,9 +20,9 @@
 // Converting a page is 16384 numbers at five instructions for four (int8), once for 256 rows.  The numbers of a group of four
 // lie in the order that conversion gives, in the queries too; the result's columns are put back at the end.
 // With n_split > 1 the walk is cut into shares, whose partials meet in scaled_merge_kernel.
-// 2048 tokens after 6144, 32 heads over 8 of 128: 331 us, 727 TFLOP/s.  A page takes 2900 cycles: 1800 of shared memory (queries,
-// keys and values read by the products, conversion), 1024 of exponentials, and the waits of softmax, products and conversion
-// for one another.
+// 2048 tokens after 6144, 32 heads over 8 of 128, int8: 341 us, 707 TFLOP/s (e4m3 294).  A page takes 2900 cycles: 1800 of shared
+// memory (queries, keys and values read by the products, conversion), 1024 of exponentials, and the waits of softmax, products
+// and conversion for one another; 16 % of the call is unequal CTAs on 148 multiprocessors.
 // Every wait is bounded; one that runs out is reported and the CTA winds down.
 #include "scaled_attention.cuh"
 
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(STC_THREADS, 1) scaled_chunk_tc_kernel(const S
     // The two warps of 32 rows leave the walk together, at a barrier of theirs (see attention_prefill_tc.cu).  A wait that ran
     // out is looked at there and not where it did: until then a tile is made of whatever is there, and nothing of it is stored.
     // (What a tile costs beside its numbers is most of the issue slots: a vote behind every wait, barriers picked by a switch, a
-    // second copy of the weights for masked tiles and a wait for P V at each tile's end made 404 us of 331.)
+    // second copy of the weights for masked tiles and a wait for P V at each tile's end: 404 us beside 331.)
     const int x = (warp - 8) >> 3, quad = warp & 3, half = ((warp - 8) & 7) >> 2, id = 4 * x + quad;
     const int row = quad * 32 + lane, rr = x * 128 + row;
     const bool live = rr < rows_here;

@@ -44,7 +44,8 @@ class LoadOptions:
     ended, as those of decode steps always do (off by default; the rule is stated in ``Engine._overlaps``).
     ``cache_dtype``: what keys and values are cached as: "" as the activations, "int8" or "float8_e4m3" as rows of 8 bits
     with a float32 scale each (a token's key or value of one kv head), which hold about twice the tokens of bfloat16 in the
-    same memory; for models whose every cached layer is attention with plain scores (``parts.attention``).
+    same memory; for models whose every cached layer is attention with plain scores (``parts.attention``).  A float32 model's queries
+    and softmax weights are multiplied with such rows in 22 bits; prompts take longer than over the activations' type.
     ``graph_prompt_tokens``: prompt steps of up to this many tokens are bound by their ~300 launches, not by
     the GPU; one whose shape comes back is captured as a CUDA graph like a decode step (0: never)."""
 

@@ -1288,7 +1288,7 @@ def scaled_attention_decode(q, out, k_cache, v_cache, k_scale, v_scale, block_ta
 
 def scaled_chunk_tc_supports(q, out, head_dim: int, scale: float) -> bool:
     """Whether the tcgen05 kernel takes the product (queries and results by 16 bytes), which it does wherever it can.  (Two tokens of 8 sequences at 2000, 32
-    heads over 8 of 128: 26 us, 37 with the other; of 16 sequences, 8 heads of 64: 34, 38 with the other.)"""
+    heads over 8 of 128: 26 us, 38 with the other; of 16 sequences, 8 heads of 64: 34, 45 with the other.)"""
     return q.dtype is torch.bfloat16 and scale > 0 and head_dim in (64, 128) and not (q.data_ptr() | out.data_ptr()) & 15
 
 
@@ -1297,8 +1297,8 @@ def scaled_chunk_shares(n_seqs: int, n_kv_heads: int, rows: int, n_pages: int, t
     """Into how many shares ``scaled_attention_chunk`` cuts every walk over the keys, by the batch's shape; ``numbers``: of the
     result.  The time is taken as waves of CTAs (one a multiprocessor, or three of the smaller kernel's), each as long as its
     pages and six more, and for several shares their partials' way through memory (8 bytes a number and share, in pages' time)
-    and a launch: one sequence of 33 tokens at 32768 takes 18 shares and 60 us, 718 in one; 2048 tokens after 6144 one
-    share, 331 us, 404 in two; 512 after 8000 two, 119 us, 196 in one."""
+    and a launch: one sequence of 33 tokens at 32768 takes 18 shares and 61 us, 744 in one; 2048 tokens after 6144 one
+    share, 341 us, 415 in two; 512 after 8000 two, 126 us, 203 in one."""
     tile, slots = (256, sms) if tc else (64, 3 * sms)
     base = n_seqs * n_kv_heads * ((rows + tile - 1) // tile)
 

@@ -14,12 +14,13 @@ ROW_DTYPES = {"int8": torch.int8, "float8_e4m3": torch.float8_e4m3fn}
 
 @dataclass
 class Runtime:
-    dtype: str                 # "bfloat16" (serving precisions) or "float32" (true 32-bit everywhere)
+    dtype: str                 # "bfloat16" (serving precisions) or "float32" (true 32-bit everywhere but over 8-bit rows, see row_dtype)
     device: torch.device
     max_positions: int         # longest sequence the cache allows; sizes position tables
     tensor_cores: bool = True  # bfloat16 only: use the tcgen05 kernels where they apply (attention over 8-bit rows: mma.sync otherwise)
     shared: dict = field(default_factory=dict)  # objects that parts of one model share (position tables)
-    # what keys and values are cached as: None as the activations, or 8-bit rows with a scale each (see ROW_DTYPES)
+    # what keys and values are cached as: None as the activations, or 8-bit rows with a scale each (see ROW_DTYPES); float32 queries
+    # and softmax weights meet such rows in 22 bits (two float16 terms), sums stay float32
     row_dtype: Optional[torch.dtype] = None
     n_sm: int = 0              # streaming multiprocessors of the device (asked once; the split policies size grids by it)
 
