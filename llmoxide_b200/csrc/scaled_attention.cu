@@ -16,6 +16,10 @@
 __device__ __forceinline__ void sat_cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+// The same, or zeros.
+__device__ __forceinline__ void sat_cp_async16(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
 __device__ __forceinline__ void sat_mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -552,12 +556,17 @@ LLMX_API int llmx_scaled_attention_decode(const void* q, void* out, int f32, con
 // (token, head of the kv head) pairs, token after token, so that a few tokens fill a tile with the heads that share their
 // keys; a CTA of four warps takes 64 of them, 16 a warp, and walks the visible keys a page of 64 at a time.  All four
 // warps convert every cached byte for 16 rows, which is what bounds it: 2048 tokens after 6144, 32 heads over 8 of 128, take
-// 1570 us (154 TFLOP/s) where the tcgen05 kernel, which converts once for 256 rows, takes 341.  With n_split > 1 the walk is cut into shares whose partials meet in scaled_merge_kernel.
+// 1470 us (164 TFLOP/s) where the tcgen05 kernel, which converts once for 256 rows, takes 341.  The weights' reference lags by up to
+// 2^5.5 (a row's largest lies between 2^10 and 2^15.5), so that most pages neither look for the largest weight nor rescale (1570 us
+// where each does; 512 float32 tokens after 2048 206, 216).  With n_split > 1 the walk is cut into shares whose partials meet in
+// scaled_merge_kernel.
 // ---------------------------------------------------------------------------
 #define SAC_WARPS 4
 #define SAC_ROWS (16 * SAC_WARPS)
 #define SAC_KEYS LLMX_PAGE
 #define SAC_MAX_SPLIT 64
+#define SAC_LAG 5.5f                         // a row's largest weight may outgrow the one it is taken against by 2^5.5,
+#define SAC_WEIGHT_POWER 10                  // which comes to 2^10: below 2^15.5, float16 ends at 2^16
 
 template <int DP, int TERMS>
 struct SacSmem {
@@ -598,11 +607,12 @@ __global__ void __launch_bounds__(SAC_WARPS * 32) scaled_chunk_kernel(const SatA
   const int pieces = D / 16;
   auto load_tile = [&](int place, int stage) {
     const size_t row = ((size_t)sat_page(a, pages, tile_at(place)) * G + g) * LLMX_PAGE;
+    const int live = FMT == ROWS_E4M3 ? pos_hi + 1 - tile_at(place) * SAC_KEYS : SAC_KEYS;      // (NaN codes past the end)
     const uint32_t sK = base + stage * S::STAGE, sV = sK + S::TILE, sS = base + S::SCALES + stage * 2 * SAC_KEYS * 4;
     for (int i = threadIdx.x; i < SAC_KEYS * pieces; i += SAC_WARPS * 32) {
       const int r = i / pieces, c = i % pieces;
       sat_cp_async16(sK + sat_at<DP, SAC_KEYS>(r, c), a.k + (row + r) * D + c * 16);
-      sat_cp_async16(sV + sat_at<DP, SAC_KEYS>(r, c), a.v + (row + r) * D + c * 16);
+      sat_cp_async16(sV + sat_at<DP, SAC_KEYS>(r, c), a.v + (row + r) * D + c * 16, r < live);
     }
     if (threadIdx.x < 16) sat_cp_async16(sS + threadIdx.x * 16, a.ks + row + threadIdx.x * 4);
     else if (threadIdx.x < 32) sat_cp_async16(sS + threadIdx.x * 16, a.vs + row + (threadIdx.x - 16) * 4);
@@ -668,6 +678,8 @@ __global__ void __launch_bounds__(SAC_WARPS * 32) scaled_chunk_kernel(const SatA
   }
   __syncwarp();
 
+  // m: log2 of the row's largest weight, a while ago; l: this lane's share of the row sum in units of 2^(m - shift)
+  constexpr float shift = TERMS == 1 ? SAC_WEIGHT_POWER : 0.f, up = TERMS == 1 ? 1.f : 1 << SAC_WEIGHT_POWER;
   float o[NJ][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
   for (int j = 0; j < NJ; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
@@ -678,13 +690,6 @@ __global__ void __launch_bounds__(SAC_WARPS * 32) scaled_chunk_kernel(const SatA
     asm volatile("cp.async.wait_group 1;" ::: "memory");
     __syncthreads();
     const int key0 = tile_at(lo + t) * SAC_KEYS;
-    if (FMT == ROWS_E4M3 && key0 + SAC_KEYS - 1 > pos_hi) {           // the last page of the CTA's walk
-      for (int i = threadIdx.x; i < SAC_KEYS * pieces; i += SAC_WARPS * 32) {
-        const int r = i / pieces;
-        if (key0 + r > pos_hi) *reinterpret_cast<uint4*>(smem + stage * S::STAGE + S::TILE + sat_at<DP, SAC_KEYS>(r, i % pieces)) = make_uint4(0u, 0u, 0u, 0u);
-      }
-      __syncthreads();
-    }
     const uint32_t sK = base + stage * S::STAGE, sV = sK + S::TILE, sS = base + S::SCALES + stage * 2 * SAC_KEYS * 4;
     float s[8][4];                                  // rows gq and gq + 8, keys 8 i + 2 tq and + 1
 #pragma unroll
@@ -721,31 +726,46 @@ __global__ void __launch_bounds__(SAC_WARPS * 32) scaled_chunk_kernel(const SatA
           if ((key >= first[r] || key < a.keep_first) && key <= at[r]) seen |= 1u << (4 * i + e);
         }
     }
-    float mx[2] = {-INFINITY, -INFINITY};
+    float mx[2] = {-INFINITY, -INFINITY}, loudest = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint2 kk = sat_lds64(sS + 4 * (8 * i + 2 * tq));
       const uint2 vv = sat_lds64(sS + 4 * (SAC_KEYS + 8 * i + 2 * tq));
       const float k0 = __uint_as_float(kk.x), k1 = __uint_as_float(kk.y);
-      const float log0 = rows_log2(__uint_as_float(vv.x)), log1 = rows_log2(__uint_as_float(vv.y));
+      loudest = fmaxf(loudest, fmaxf(fabsf(__uint_as_float(vv.x)), fabsf(__uint_as_float(vv.y))));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         s[i][e] = (seen >> (4 * i + e)) & 1u ? s[i][e] * ((e & 1 ? k1 : k0) * unit[e >> 1]) : -INFINITY;
-        mx[e >> 1] = fmaxf(mx[e >> 1], s[i][e] + (e & 1 ? log1 : log0));
+        mx[e >> 1] = fmaxf(mx[e >> 1], s[i][e]);
       }
     }
-    float ref[2], c[2], sum[2] = {0.f, 0.f};
+    // no weight of this lane's is above its largest score times its loudest value (seen or not); where that is far enough above
+    // a row's reference, the largest weight itself is looked for
+    loudest = rows_log2(loudest);
+    if (__any_sync(0xffffffffu, mx[0] + loudest > m[0] + SAC_LAG || mx[1] + loudest > m[1] + SAC_LAG)) {
+      mx[0] = mx[1] = -INFINITY;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-      mx[r] = fmaxf(mx[r] - sat_weight_shift<TERMS>(), m[r]);
-      ref[r] = mx[r] == -INFINITY ? 0.f : mx[r];    // a row that has seen nothing yet
-      c[r] = sat_exp2<TERMS>(m[r] - ref[r]);
-      m[r] = mx[r];
+      for (int i = 0; i < 8; ++i) {
+        const uint2 vv = sat_lds64(sS + 4 * (SAC_KEYS + 8 * i + 2 * tq));
+        const float log0 = rows_log2(__uint_as_float(vv.x)), log1 = rows_log2(__uint_as_float(vv.y));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], s[i][e] + (e & 1 ? log1 : log0));
+      }
+      float c[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+        c[r] = 1.f;
+        if (mx[r] > m[r] + SAC_LAG) c[r] = sat_exp2<TERMS>(m[r] - mx[r]), m[r] = mx[r];
+        l[r] *= c[r];
+      }
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) o[j][0] *= c[0], o[j][1] *= c[0], o[j][2] *= c[1], o[j][3] *= c[1];
     }
+    float ref[2], sum[2] = {0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) o[j][0] *= c[0], o[j][1] *= c[0], o[j][2] *= c[1], o[j][3] *= c[1];
+    for (int r = 0; r < 2; ++r) ref[r] = m[r] == -INFINITY ? 0.f : m[r] - shift;      // (nothing seen yet)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {                   // sixteen keys at a time
       uint32_t pa[TERMS][4];
@@ -759,7 +779,7 @@ __global__ void __launch_bounds__(SAC_WARPS * 32) scaled_chunk_kernel(const SatA
           sum[r] += p0 + p1;
           const uint32_t vis = seen >> (4 * (2 * i + x) + 2 * r);
           uint32_t terms[TERMS];
-          rows_split2<TERMS>(vis & 1u ? p0 * w0 * sat_weight_mul<TERMS>() : 0.f, vis & 2u ? p1 * w1 * sat_weight_mul<TERMS>() : 0.f, terms);
+          rows_split2<TERMS>(vis & 1u ? p0 * w0 * up : 0.f, vis & 2u ? p1 * w1 * up : 0.f, terms);
 #pragma unroll
           for (int e = 0; e < TERMS; ++e) pa[e][2 * x + r] = terms[e];
         }
@@ -801,7 +821,7 @@ __global__ void __launch_bounds__(SAC_WARPS * 32) scaled_chunk_kernel(const SatA
 #undef SAC_DIMS
     }
 #pragma unroll
-    for (int r = 0; r < 2; ++r) l[r] = l[r] * c[r] + sum[r];
+    for (int r = 0; r < 2; ++r) l[r] += sum[r];
     __syncthreads();                                // the stage is refilled by the next iteration's copies
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -811,7 +831,7 @@ __global__ void __launch_bounds__(SAC_WARPS * 32) scaled_chunk_kernel(const SatA
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     if (!live[r]) continue;
     const size_t row = (size_t)(tok0 + token[r]) * H + head[r];
-    const float f = (a.n_split > 1 ? 1.f : l[r] == 0.f ? 0.f : 1.f / l[r]) / sat_weight_mul<TERMS>();
+    const float f = (a.n_split > 1 ? 1.f : l[r] == 0.f ? 0.f : 1.f / l[r]) / up;
     float* part = a.ws + (row * a.n_split + share) * SAT_WS_ROW(D);
     constexpr int RUN = DP == 64 ? 8 : 16;          // neighbouring dims of a lane: columns 2 tq and 2 tq + 1 of the products
 #pragma unroll
@@ -824,7 +844,7 @@ __global__ void __launch_bounds__(SAC_WARPS * 32) scaled_chunk_kernel(const SatA
         if (a.n_split > 1) *reinterpret_cast<float4*>(part + d) = v;
         else sat_store4<TERMS>(a.out, row * D + d, v);
       }
-    if (a.n_split > 1 && tq == 0) part[D] = m[r], part[D + 1] = l[r];
+    if (a.n_split > 1 && tq == 0) part[D] = m[r] - shift, part[D + 1] = l[r];
   }
 }
 

@@ -26,7 +26,7 @@ __device__ __forceinline__ float sat_largest(float top, float4 f) {
   const uint32_t b = max(__float_as_uint(f.z) & 0x7fffffffu, __float_as_uint(f.w) & 0x7fffffffu);
   return __uint_as_float(max(__float_as_uint(top), max(a, b)));
 }
-// Weights at 2^13 (ROWS_WEIGHT_POWER): by the reference where they are rounded once; by a factor of its own where float32 is kept
+// Single tokens' weights at 2^13 (ROWS_WEIGHT_POWER): by the reference where they are rounded once; by a factor of its own where float32 is kept
 // in two terms, since an argument of the exponential that is larger by 13 costs it a digit and a half.
 template <int TERMS> __device__ __forceinline__ constexpr float sat_weight_shift() { return TERMS == 1 ? ROWS_WEIGHT_POWER : 0.f; }
 template <int TERMS> __device__ __forceinline__ constexpr float sat_weight_mul() { return TERMS == 1 ? 1.f : 8192.f; }

@@ -1,7 +1,7 @@
 // Attention of several new tokens per sequence over the cache of 8-bit rows on the 5th-generation tensor cores (tcgen05):
-// bfloat16 queries, head sizes 64 and 128.  Formulas and roundings as in scaled_attention.cu, but for the weights' reference, which
-// lags: a row's largest weight lies between 2^10 and 2^15.5, so that weights below 2^-24 of it lose digits and those below
-// 2^-35 vanish.
+// bfloat16 queries, head sizes 64 and 128.  Formulas and roundings as in scaled_attention.cu's kernel of several
+// tokens, whose weights' reference lags: a row's largest weight lies between 2^10 and 2^15.5, so that weights below 2^-24 of it
+// lose digits and those below 2^-35 vanish.
 //
 // Rows of the product are a kv head's (token, query head) pairs, token after token, so that the heads that share keys share a
 // tile, and a few tokens fill it.  A CTA owns 256 of them, as two tiles of 128 (a row = a lane of tensor memory), and walks the

@@ -1288,7 +1288,7 @@ def scaled_attention_decode(q, out, k_cache, v_cache, k_scale, v_scale, block_ta
 
 def scaled_chunk_tc_supports(q, out, head_dim: int, scale: float) -> bool:
     """Whether the tcgen05 kernel takes the product (queries and results by 16 bytes), which it does wherever it can.  (Two tokens of 8 sequences at 2000, 32
-    heads over 8 of 128: 26 us, 38 with the other; of 16 sequences, 8 heads of 64: 34, 45 with the other.)"""
+    heads over 8 of 128: 26 us, 37 with the other; of 16 sequences, 8 heads of 64: 34, 41 with the other.)"""
     return q.dtype is torch.bfloat16 and scale > 0 and head_dim in (64, 128) and not (q.data_ptr() | out.data_ptr()) & 15
 
 
